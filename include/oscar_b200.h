@@ -29,7 +29,8 @@ extern "C" {
 
 enum {
   OSCAR_OK = 0,
-  OSCAR_ERR_INVALID = 1,   /* bad argument: null pointer, size, alignment, geometry */
+  OSCAR_ERR_INVALID = 1,   /* bad argument: null pointer, size, alignment, geometry;
+                              in a status word: bad data that only the device sees    */
   OSCAR_ERR_LAUNCH = 2,    /* CUDA launch error (cudaGetLastError after launch)     */
   OSCAR_ERR_UNSUPPORTED = 3,
   OSCAR_ERR_TIMEOUT = 4    /* a bounded device wait gave up (reported via status buffer) */
@@ -261,6 +262,64 @@ int oscar_decode_attention_noalloc(const void *qrot, const void *query, int64_t 
 
 /* Row capacity of the built-in scratch of oscar_decode_attention_noalloc. */
 int64_t oscar_decode_attention_noalloc_max_rows(void);
+
+/* Norms of queries and keys per head and the position rotation, one pass (no reference
+ * counterpart: there the model does it before the backend is called).  For every token
+ * and head: y = x * rsqrt(mean(x^2) + eps) * (w + weight_offset) over the 256 dims, then
+ * the first `rotary` dims turn by the cos / sin of the token's position: pairs
+ * (i, i + rotary/2), or (2i, 2i + 1) when interleaved.  fp32 inside, one rounding to bf16.
+ * query [n, hq, 256] / key [n, hkv, 256] and their outputs: 16-byte aligned rows, strides
+ * (token, head) multiples of 8 elements; an output may be its own input (same pointer and
+ * strides) and must not overlap any other row.  q_weight / k_weight: 256 values, fp32
+ * (weight_f32) or bf16.  positions: n int64 (positions_64) or int32.  cos_sin: [max_positions,
+ * rotary] contiguous, cosines then sines, fp32 (table_f32) or bf16; rotary a multiple of 16,
+ * at most 256, 0 for none.  counts (nullable): tokens >= counts[1] are left unwritten.  A
+ * token whose position is outside the table is left unwritten and OSCAR_ERR_INVALID goes to
+ * *status (nullable). */
+int oscar_qk_norm_rope(const void *query, int64_t qs0, int64_t qs1, const void *key, int64_t ks0, int64_t ks1,
+                       int64_t n, int32_t hq, int32_t hkv, const void *q_weight, const void *k_weight,
+                       int32_t weight_f32, float weight_offset, float eps, const void *positions,
+                       int32_t positions_64, const void *cos_sin, int32_t table_f32, int64_t max_positions,
+                       int32_t rotary, int32_t interleaved, const int32_t *counts, void *query_out, int64_t qos0,
+                       int64_t qos1, void *key_out, int64_t kos0, int64_t kos1, int32_t *status, void *stream);
+
+/* ---- page pool (no reference counterpart: there the host engine owns the pages and
+ * shared pages are refused, backend.py:41-64) ----------------------------------------
+ * One caller-owned, 16-byte aligned int32 arena: reference counts [num_pages] (page 0 is
+ * never handed out and holds 1), lengths [max_reqs], block table [max_reqs, columns] in
+ * 128-token kernel blocks (unused entries 0), then workspace that the calls below share,
+ * so calls on one arena must be ordered.  A row of L tokens holds ceil(L / block_tokens)
+ * pages; fresh pages are the free pages of the lowest numbers, handed out in list order:
+ * results depend on the state and the list alone.  Writes the word offsets {counts,
+ * lengths, table, end of the state, total words} to offsets[0..4]. */
+int oscar_page_pool_layout(int32_t num_pages, int32_t max_reqs, int32_t columns, int64_t *offsets);
+
+/* Fork row children[i] from row parents[i], i < count <= max_reqs: the child holds the
+ * parent's tokens, sharing its full pages but the first (their counts grow by one); the
+ * first page (its used slots and the request's BF16 window) and a partial last page (its
+ * used slots) are copied to fresh pages.  history / window: the cache stripes of num_pages
+ * pages.  A pair is valid when the parent had tokens and the child none before the call
+ * and no earlier pair names the child.  result[i] = 1 forked, 0 not forked because the
+ * free pages ran out at this pair or before, -1 not a valid pair. */
+int oscar_fork_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, const int32_t *parents,
+                        const int32_t *children, int32_t count, void *history, void *window, oscar_geometry geo,
+                        int32_t *result, void *stream);
+
+/* Row rows[i] gets lens[i] tokens, i < count <= max_reqs: 0 releases the row (the counts of
+ * its pages drop by one), a length not below the present one adds the missing pages.  All
+ * releases of the call come before any growth.  result[i] = 1 done, 0 unchanged because the
+ * free pages ran out at this entry or before, -1 refused: row or length out of range, a
+ * shorter length other than 0, or a row that an earlier entry names. */
+int oscar_resize_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, int32_t block_tokens,
+                          const int32_t *rows, const int32_t *lens, int32_t count, int32_t *result, void *stream);
+
+/* Move the live pages onto the page numbers 1 .. live: the k-th live page above goes to the
+ * k-th free page within.  Slots that some row uses move, and the window of a row's first
+ * page; counts and table follow, table entries past a row's pages become 0.
+ * summary[0..1] = {live pages, moved pages}; moved_to[num_pages] = each page's new number,
+ * -1 for a page that was free. */
+int oscar_compact_pages(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, void *history,
+                        void *window, oscar_geometry geo, int32_t *summary, int32_t *moved_to, void *stream);
 
 /* ---- calibration (reference oscar_ascend/calibration_kernels.py) -------------- */
 

@@ -951,13 +951,6 @@ __global__ void __launch_bounds__(1024) prepare_tasks_kernel(const int32_t *__re
 // ----------------------------------------------------------------------------
 // launch helpers
 // ----------------------------------------------------------------------------
-static bool geo_ok(const oscar_geometry &g) {
-  return g.head_dim == kDim && g.kv_heads > 0 && g.group > 0 && g.kernel_block == kKernelBlock &&
-         g.block_tokens % kKernelBlock == 0 && g.slot_bytes % 16 == 0 && g.vector_bytes == kDataBytes + 4 &&
-         g.page_bytes == (int64_t)g.block_tokens * g.kv_heads * kDim * 2 && g.ring > 0 && g.sink >= 0 &&
-         g.recent >= 0 && g.query_tile > 0 && g.table_stride > 0;
-}
-
 // priority != 0: launch priority of the grid (the decode step gives the history grid the
 // device's greatest priority, so a concurrently queued lower-priority grid only takes
 // the SM slots that history blocks leave free, i.e. the tail of the last wave)
@@ -1147,7 +1140,7 @@ extern "C" int oscar_attention_partials(const void *query, int64_t qs0, int64_t 
                                         const int32_t *tasks, const int32_t *task_count, int32_t num_tasks,
                                         int64_t n, float *partials, float *lse, oscar_geometry geo, float scale,
                                         int32_t splits, int32_t raw, int32_t *status, void *stream) {
-  if (!geo_ok(geo) || splits <= 0 || num_tasks < 0 || n < 0) return OSCAR_ERR_INVALID;
+  if (!paged_geometry_ok(geo) || splits <= 0 || num_tasks < 0 || n < 0) return OSCAR_ERR_INVALID;
   if (n == 0 || num_tasks == 0) return OSCAR_OK;
   if (!query || !qstarts || !seq_lens || !table || !counts || !tasks || !task_count || !partials || !lse)
     return OSCAR_ERR_INVALID;
@@ -1216,7 +1209,7 @@ extern "C" int oscar_store_windows(const void *key, int64_t ks0, int64_t ks1, co
                                    int64_t vs1, void *window, const int32_t *qstarts, const int32_t *seq_lens,
                                    const int32_t *table, const int32_t *counts, int32_t num_programs,
                                    oscar_geometry geo, void *stream) {
-  if (!geo_ok(geo) || num_programs < 0) return OSCAR_ERR_INVALID;
+  if (!paged_geometry_ok(geo) || num_programs < 0) return OSCAR_ERR_INVALID;
   if (num_programs == 0) return OSCAR_OK;
   if (!key || !value || !window || !qstarts || !seq_lens || !table || !counts) return OSCAR_ERR_INVALID;
   if (((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) || ks0 % 8 || ks1 % 8 ||
@@ -1237,7 +1230,7 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
                                       const void *rv, float *scratch_partials, float *scratch_lse, void *output,
                                       oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
                                       int32_t *status, void *stream) {
-  if (!geo_ok(geo) || splits <= 0 || splits > 64 || num_tasks < 0 || n < 0 || window_programs < 0)
+  if (!paged_geometry_ok(geo) || splits <= 0 || splits > 64 || num_tasks < 0 || n < 0 || window_programs < 0)
     return OSCAR_ERR_INVALID;  // the fused merge holds at most 64 split LSEs per row in one warp
   if (n == 0) return OSCAR_OK;
   if (!qrot || !query || !key || !value || !history || !window || !qstarts || !seq_lens || !table || !counts ||

@@ -217,6 +217,14 @@ OSCAR_DEVINL int window_index(int pos, const oscar_geometry &g) {
   return pos < g.sink ? pos : g.sink + pos % g.ring;
 }
 
+// Geometry rules of the paged entry points (host).
+inline bool paged_geometry_ok(const oscar_geometry &g) {
+  return g.head_dim == kDim && g.kv_heads > 0 && g.group > 0 && g.kernel_block == kKernelBlock &&
+         g.block_tokens % kKernelBlock == 0 && g.slot_bytes % 16 == 0 && g.vector_bytes == kDataBytes + 4 &&
+         g.page_bytes == (int64_t)g.block_tokens * g.kv_heads * kDim * 2 && g.ring > 0 && g.sink >= 0 &&
+         g.recent >= 0 && g.query_tile > 0 && g.table_stride > 0;
+}
+
 }  // namespace oscar
 
 // Opt kernel `Kernel` into `bytes` of dynamic shared memory on the current device.  The

@@ -12,6 +12,7 @@ uses them.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -251,6 +252,184 @@ def prefill_attention(query, key, value, query_start_loc, num_reqs: int, max_que
               query_start_loc.data_ptr(), num_reqs, max_query_len, n, hq, key.shape[1], float(scale), out.data_ptr(),
               out.stride(0), out.stride(1), _status(out), _stream(query))
     return out
+
+
+def _same_device(*tensors):
+    """All on one CUDA device; returns the context that makes it current if it is not."""
+    _require_cuda(*tensors)
+    given = [t for t in tensors if t is not None]
+    device = given[0].device
+    if any(t.device != device for t in given):
+        raise ValueError(f"tensors on several devices: {sorted({str(t.device) for t in given})}")
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _output_rows(out, like):
+    """``out`` (or a new tensor) as the bf16 rows a kernel writes for ``like``."""
+    if out is None:
+        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+    if out.dtype != torch.bfloat16 or out.shape != like.shape:
+        raise ValueError(f"expected a bf16 output of shape {tuple(like.shape)}, got {tuple(out.shape)} {out.dtype}")
+    if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+        raise ValueError("output rows must be 16-byte aligned with unit inner stride")
+    n, h, _ = out.shape
+    if (n > 1 and h > 1 and abs(out.stride(0)) < 256 and abs(out.stride(1)) < 256) or (
+            n > 1 and out.stride(0) == 0) or (h > 1 and out.stride(1) == 0):
+        raise ValueError("output rows overlap each other")
+    return out
+
+
+def _rows_apart(a, b) -> bool:
+    """Whether two [n, h, 256] row sets cannot share memory: apart altogether, or columns of
+    one fused [n, width] buffer that do not meet."""
+    def span(t):
+        n, h, _ = t.shape
+        return t.data_ptr(), t.data_ptr() + 2 * ((n - 1) * t.stride(0) + (h - 1) * t.stride(1) + 256)
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    step = 2 * a.stride(0)
+    if a.shape[0] != b.shape[0] or step != 2 * b.stride(0) or step <= 0:
+        return False
+    wide = [2 * ((t.shape[1] - 1) * t.stride(1) + 256) for t in (a, b)]
+    gap = (b0 - a0) % step
+    return max(wide) <= step and gap >= wide[0] and gap + wide[1] <= step
+
+
+def qk_norm_rope(query, key, q_weight, k_weight, positions, cos_sin, eps=1e-6, weight_offset=0.0, interleaved=False,
+                 counts=None, query_out=None, key_out=None):
+    """Norm of every query and key head and the rotation of its position, in one pass.
+
+    query [n, Hq, 256] and key [n, Hkv, 256] bf16, any strides with unit inner stride (views
+    of a fused projection); weights [256] and the table cos_sin [positions, rotary]
+    (cosines, then sines) fp32 or bf16; positions int64 or int32 [n].
+    ``y = x * rsqrt(mean(x^2) + eps) * (w + weight_offset)``, then the first ``rotary`` dims
+    turn: pairs (i, i + rotary/2), or (2i, 2i+1) with ``interleaved``.  fp32 inside (a row's
+    sum of squares has to fit: elements up to about 2^59).
+    Outputs are new tensors, or ``query_out`` / ``key_out``: an output may be its own input,
+    and must otherwise not overlap the other rows.  ``counts`` (device [requests, active
+    tokens]) leaves the tokens behind the active ones as they were.  A token whose position
+    is not in the table stays unwritten and raises the status word (``read_status`` = 1).
+    Returns (query_out, key_out)."""
+    for t, name in ((query, "query"), (key, "key")):
+        if t.ndim != 3 or t.dtype != torch.bfloat16 or t.shape[2] != 256:
+            raise ValueError(f"{name}: expected bf16 [n, heads, 256], got {tuple(t.shape)} {t.dtype}")
+    n = query.shape[0]
+    if key.shape[0] != n or positions.shape != (n,):
+        raise ValueError("query, key and positions must have the same tokens")
+    if q_weight.shape != (256,) or k_weight.shape != (256,) or q_weight.dtype != k_weight.dtype:
+        raise ValueError("norm weights are [256], both of one type")
+    if cos_sin.ndim != 2 or cos_sin.shape[1] % 16 or cos_sin.shape[1] > 256:
+        raise ValueError("the cos / sin table is [positions, rotary], rotary a multiple of 16 up to 256")
+    for t, name in ((q_weight, "weights"), (cos_sin, "table")):
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{name} must be fp32 or bf16, got {t.dtype}")
+    if positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError("positions must be int64 or int32")
+    if counts is not None and (counts.dtype != torch.int32 or counts.numel() < 2):
+        raise ValueError("counts are int32 [requests, active tokens]")
+    if not float(eps) >= 0.0:
+        raise ValueError("eps must not be negative")
+    qo, ko = _output_rows(query_out, query), _output_rows(key_out, key)
+    if query_out is not None or key_out is not None:
+        same = [o.data_ptr() == i.data_ptr() and o.stride() == i.stride() for o, i in ((qo, query), (ko, key))]
+        pairs = [(qo, ko), (qo, key), (ko, query)] + [p for p, s in zip(((qo, query), (ko, key)), same) if not s]
+        if not all(0 in a.shape or 0 in b.shape or _rows_apart(a, b) for a, b in pairs):
+            raise ValueError("an output overlaps rows other than its own input's")
+    device = _same_device(query, key, q_weight, k_weight, positions, cos_sin, counts, query_out, key_out)
+    if n == 0:
+        return qo, ko
+    query, key = _rows(query), _rows(key)
+    aligned = [t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+               for t in (q_weight, k_weight, cos_sin, positions)]
+    with device:
+        _lib.call("oscar_qk_norm_rope", query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(),
+                  key.stride(0), key.stride(1), n, query.shape[1], key.shape[1], aligned[0].data_ptr(),
+                  aligned[1].data_ptr(), int(q_weight.dtype == torch.float32), float(weight_offset), float(eps),
+                  aligned[3].data_ptr(), int(positions.dtype == torch.int64), aligned[2].data_ptr(),
+                  int(cos_sin.dtype == torch.float32), cos_sin.shape[0], cos_sin.shape[1], int(bool(interleaved)),
+                  _ptr(counts), qo.data_ptr(), qo.stride(0), qo.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1),
+                  _status(query), _stream(query))
+    _checked("oscar_qk_norm_rope", query)
+    return qo, ko
+
+
+# ----------------------------------------------------------------------------
+# page pool (``pages.PagePool``)
+# ----------------------------------------------------------------------------
+
+
+def page_pool_layout(num_pages: int, max_reqs: int, columns: int) -> dict:
+    """Word offsets of a page pool's arena (host-only call, no device)."""
+    off = (C.c_int64 * 5)()
+    _lib.call("oscar_page_pool_layout", num_pages, max_reqs, columns, C.addressof(off))
+    return dict(zip(("refcounts", "lens", "table", "state", "words"), (int(x) for x in off)))
+
+
+def _pool_list(pool, *lists):
+    """int32 device lists of one length, at most one entry per row of the pool."""
+    for t in lists:
+        if t.dtype != torch.int32 or t.ndim != 1 or t.shape != lists[0].shape:
+            raise ValueError("row lists are int32 [count], all of one length")
+    if lists[0].shape[0] > pool.max_reqs:
+        raise ValueError(f"{lists[0].shape[0]} entries for a pool of {pool.max_reqs} rows")
+    return [t.contiguous() for t in lists]
+
+
+def fork_requests(pool, parents, children, history, window):
+    """Fork rows of a page pool copy-on-write: row ``children[i]`` gets the tokens of row
+    ``parents[i]`` (int32 device lists).
+
+    Full pages but the first are shared; the first page's used slots and BF16 window and a
+    partial last page's used slots are copied to fresh pages of the cache (``history`` /
+    ``window``, the flat views of ``CacheLayout.tensor_views``).  Returns int32 [count]: 1
+    forked; 0 the free pages ran out at this pair or before; -1 not a valid pair (an empty
+    or unknown parent, a child that holds tokens or that an earlier pair names)."""
+    pool.check_stripes(history, window)
+    parents, children = _pool_list(pool, parents, children)
+    device = _same_device(pool.arena, parents, children, history, window)
+    result = torch.empty(parents.shape, dtype=torch.int32, device=parents.device)
+    with device:
+        _lib.call("oscar_fork_requests", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
+                  parents.data_ptr(), children.data_ptr(), parents.shape[0], history.data_ptr(), window.data_ptr(),
+                  pool.geometry, result.data_ptr(), _stream(parents))
+    return result
+
+
+def resize_requests(pool, rows, lens):
+    """Admit, grow and release rows of a page pool: row ``rows[i]`` gets ``lens[i]`` tokens
+    (int32 device lists), 0 to release it.
+
+    Releases come before growth, so their pages serve the same call.  Returns int32
+    [count]: 1 done; 0 the free pages ran out at this entry or before (the row is
+    unchanged); -1 refused (row or length out of range, a shorter length other than 0, a
+    row that an earlier entry names)."""
+    rows, lens = _pool_list(pool, rows, lens)
+    device = _same_device(pool.arena, rows, lens)
+    result = torch.empty(rows.shape, dtype=torch.int32, device=rows.device)
+    with device:
+        _lib.call("oscar_resize_requests", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
+                  pool.layout.physical_block_tokens, rows.data_ptr(), lens.data_ptr(), rows.shape[0],
+                  result.data_ptr(), _stream(rows))
+    return result
+
+
+def compact_pages(pool, history, window):
+    """Move a pool's live pages onto the lowest page numbers (1 .. live), with the slots and
+    windows they hold; counts and table follow.  Returns (summary int32 [live pages, moved
+    pages], moved_to int32 [num_pages]: each page's new number, -1 for a free page)."""
+    pool.check_stripes(history, window)
+    device = _same_device(pool.arena, history, window)
+    summary = torch.empty(2, dtype=torch.int32, device=pool.device)
+    moved_to = torch.empty(pool.num_pages, dtype=torch.int32, device=pool.device)
+    with device:
+        _lib.call("oscar_compact_pages", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
+                  history.data_ptr(), window.data_ptr(), pool.geometry, summary.data_ptr(), moved_to.data_ptr(),
+                  _stream(summary))
+    return summary, moved_to
 
 
 def _meta_common(meta, layout, hq):

@@ -1,0 +1,143 @@
+"""Page pool operators against the plain model: state, results and every byte of the cache
+are equal."""
+
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from oscar_new_b200 import kernels
+from oscar_new_b200.layout import CacheLayout
+from oscar_new_b200.pages import PagePool
+from oscar_new_b200.synthetic import cache_stripes
+from tests.helpers import make_config
+from tests.pool_model import PoolModel
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+class Pair:
+    """A pool and its model over one cache."""
+
+    def __init__(self, pages, rows, tokens, layout, seed=0):
+        columns = -(-tokens // layout.physical_block_tokens) * layout.blocks_per_page
+        self.pool, self.model = PagePool(pages, rows, columns, layout, DEV), PoolModel(pages, rows, columns, layout)
+        cache = cache_stripes(pages, layout.physical_block_tokens, layout.kv_heads, DEV)
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        cache.view(torch.int16).random_(generator=g)
+        self.history, self.window = layout.tensor_views(cache)
+        self.h = self.history.cpu().numpy().copy()
+        self.w = self.window.view(torch.uint8).cpu().numpy().copy()
+
+    def ints(self, x):
+        return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+    def resize(self, rows, lens):
+        got = kernels.resize_requests(self.pool, self.ints(rows), self.ints(lens))
+        assert got.tolist() == self.model.resize(rows, lens)
+        self.state()
+
+    def fork(self, parents, children):
+        got = kernels.fork_requests(self.pool, self.ints(parents), self.ints(children), self.history, self.window)
+        want, copies = self.model.fork(parents, children)
+        assert got.tolist() == want
+        self.model.copy(self.h, self.w, copies)
+        self.state()
+        self.bytes()
+
+    def compact(self):
+        summary, to = kernels.compact_pages(self.pool, self.history, self.window)
+        live, want, copies = self.model.compact()
+        assert summary.tolist() == [live, len(copies)] and to.tolist() == want
+        self.model.copy(self.h, self.w, copies)
+        self.state()
+        self.bytes()
+
+    def state(self):
+        assert self.pool.refcounts.tolist() == self.model.refs and self.pool.seq_lens.tolist() == self.model.lens
+        assert np.array_equal(self.pool.block_tables.cpu().numpy(), self.model.table())
+
+    def bytes(self):
+        assert np.array_equal(self.history.cpu().numpy(), self.h)
+        assert np.array_equal(self.window.view(torch.uint8).cpu().numpy(), self.w)
+
+
+@pytest.mark.parametrize("block,heads,sink,recent,mtp", [(768, 4, 64, 256, 3), (128, 1, 0, 8, 0), (256, 3, 4, 64, 0)])
+def test_random_steps(cuda_lib, block, heads, sink, recent, mtp):
+    layout = CacheLayout(block, kv_heads=heads, config=make_config(sink, recent, mtp))
+    p, rng = Pair(23, 9, 5 * block, layout), random.Random(block)
+    for step in range(40):
+        kind = rng.random()
+        k = rng.randint(1, 9)
+        rows = [rng.randint(-1, 9) for _ in range(k)]
+        if kind < 0.5:
+            p.resize(rows, [rng.choice([0, rng.randint(1, 5 * block + 3), block * rng.randint(1, 5), 1, -7])
+                            for _ in range(k)])
+        elif kind < 0.85:
+            p.fork([rng.randint(-1, 9) for _ in range(k)], rows)
+        else:
+            p.compact()
+
+
+@pytest.mark.parametrize("tokens", [1, 127, 767, 768, 769, 1536, 1537, 3000])
+def test_fork_lengths_around_the_page_edges(cuda_lib, tokens):
+    layout = CacheLayout(768, kv_heads=2, config=make_config(4, 64))
+    p = Pair(40, 8, 3072, layout, seed=tokens)
+    p.resize([5, 2], [tokens, 900])
+    p.fork([5, 5, 2, 5], [0, 1, 3, 7])
+    p.fork([0, 7], [4, 6])  # forks of forks
+    p.resize([5, 0], [0, min(tokens + 800, 3072)])  # the first parent ends, its children live on
+    p.compact()
+
+
+def test_pages_run_out_in_list_order(cuda_lib):
+    layout = CacheLayout(256, kv_heads=1, config=make_config(4, 64))
+    p = Pair(8, 6, 2048, layout)
+    p.resize([0, 1, 2, 3], [600, 512, 600, 1])  # 3 + 2 + 3 pages of 7: the last two entries fail
+    assert p.pool.seq_lens.tolist() == [600, 512, 0, 0, 0, 0]
+    p.fork([0, 1, 0], [2, 3, 4])  # two pages left: one fork of 0
+    p.resize([0, 4], [0, 256])  # the released pages serve the same call
+    p.resize([1, 1, 2], [512, 0, 601])  # no page needed; the second naming of row 1 is refused
+
+
+def test_many_rows_and_pages(cuda_lib):
+    """More list entries than one block's threads and more pages than one scan step."""
+    layout = CacheLayout(128, kv_heads=1, config=make_config(0, 4))
+    rng = random.Random(1)
+    p = Pair(9000, 2500, 640, layout)
+    order = list(range(2500))
+    rng.shuffle(order)
+    p.resize(order, [rng.randint(1, 640) if r < 2000 else 0 for r in order])
+    p.fork([rng.randint(0, 2100) for _ in range(600)], [rng.randint(1990, 2499) for _ in range(600)])
+    p.resize(order[:1700], [0] * 1700)
+    p.compact()
+    p.resize(list(range(2500)), [640] * 2500)
+
+
+def test_captured_steps_replay_on_new_lists(cuda_lib):
+    layout = CacheLayout(256, kv_heads=2, config=make_config(4, 64))
+    p = Pair(30, 6, 2048, layout)
+    a, b = p.ints([0, 0]), p.ints([1, 2])
+    r, n = p.ints([0, 3]), p.ints([700, 300])
+    kernels.resize_requests(p.pool, p.ints([]), p.ints([]))  # nothing to do
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grown = kernels.resize_requests(p.pool, r, n)
+        forked = kernels.fork_requests(p.pool, a, b, p.history, p.window)
+        summary, to = kernels.compact_pages(p.pool, p.history, p.window)
+    for lists in (([0, 3], [700, 300], [0, 0], [1, 2]), ([1, 2], [0, 900], [3, 0], [4, 1]), ([0, 5], [0, 1], [0, 5], [1, 0])):
+        for t, v in zip((r, n, a, b), lists):
+            t.copy_(p.ints(v))
+        graph.replay()
+        want = p.model.resize(lists[0], lists[1])
+        wanted, copies = p.model.fork(lists[2], lists[3])
+        p.model.copy(p.h, p.w, copies)
+        live, where, copies = p.model.compact()
+        p.model.copy(p.h, p.w, copies)
+        assert grown.tolist() == want and forked.tolist() == wanted
+        assert summary.tolist() == [live, len(copies)] and to.tolist() == where
+        p.state()
+        p.bytes()
