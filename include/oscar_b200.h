@@ -283,6 +283,41 @@ int oscar_qk_norm_rope(const void *query, int64_t qs0, int64_t qs1, const void *
                        int32_t rotary, int32_t interleaved, const int32_t *counts, void *query_out, int64_t qos0,
                        int64_t qos1, void *key_out, int64_t kos0, int64_t kos1, int32_t *status, void *stream);
 
+/* ---- decode of requests that share prefixes (no reference counterpart: there shared
+ * prefixes are refused, metadata.py:84-87) --------------------------------------------
+ * Consecutive requests of a step with the same label groups[r] >= 0 form a group: their
+ * first prefix_lens[r] tokens (the shortest counts) hold the same packed history, e.g. as
+ * pages that oscar_fork_requests shares.  The plan covers, per group of at least two
+ * active requests, the history positions [sink, end) with end the shortest of the members'
+ * prefix lengths and starts of their BF16 recent windows; the rest of each request's
+ * history, and every request outside a group, goes the way of oscar_decode_attention.
+ *
+ * Sizes of a plan for steps of at most max_reqs (<= 8192) requests and `tokens` tokens:
+ * sizes[0] = work items, sizes[1] = int32 words.  A step with more row tiles than the plan
+ * holds is computed without sharing. */
+int oscar_shared_prefix_layout(int32_t max_reqs, int64_t tokens, int32_t hq, int32_t kv_heads, int64_t *sizes);
+
+/* Fill the plan (16-byte aligned) of one step from its device metadata, in one launch:
+ * once per step, for all layers.  groups / prefix_lens: int32 [max_reqs].  A group's
+ * history is cut into at most `splits` (1..63) parts. */
+int oscar_prepare_shared_prefix(const int32_t *qstarts, const int32_t *seq_lens, const int32_t *counts,
+                                const int32_t *groups, const int32_t *prefix_lens, int32_t max_reqs, int32_t items,
+                                int32_t splits, oscar_geometry geo, int32_t *plan, void *stream);
+
+/* oscar_decode_attention for a step with a plan: num_pages pages of the cache, the plan
+ * with the capacities and split count it was filled with (splits + plan_splits <= 64),
+ * scale > 0.  Scratch rows hold splits + plan_splits + 1 partials.  The merged history row
+ * is kept to about 16 bits through the inverse rotation and the output rounded once. */
+int oscar_decode_attention_shared(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key,
+                                  int64_t ks0, int64_t ks1, const void *value, int64_t vs0, int64_t vs1,
+                                  const uint8_t *history, int64_t num_pages, void *window, const int32_t *qstarts,
+                                  const int32_t *seq_lens, const int32_t *table, const int32_t *counts,
+                                  const int32_t *tasks, const int32_t *task_count, int32_t num_tasks, int64_t n,
+                                  const void *rv, const int32_t *plan, int32_t plan_reqs, int32_t plan_items,
+                                  int32_t plan_splits, float *scratch_partials, float *scratch_lse, void *output,
+                                  oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
+                                  int32_t *status, void *stream);
+
 /* ---- page pool (no reference counterpart: there the host engine owns the pages and
  * shared pages are refused, backend.py:41-64) ----------------------------------------
  * One caller-owned, 16-byte aligned int32 arena: reference counts [num_pages] (page 0 is

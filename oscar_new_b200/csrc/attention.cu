@@ -30,6 +30,7 @@
 #include <mutex>
 
 #include "history_common.cuh"
+#include "shared_prefix.cuh"
 #include "tasks.cuh"
 #include "rowgemm.cuh"
 
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(32 * MAXW, MINB) history_attention_kernel(Hist
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int task = blockIdx.x, split = blockIdx.y;
   const int h0 = blockIdx.z * P.heads_per_cta;
-  const TaskInfo ti = load_task(task, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+  const TaskInfo ti = load_history_task(task, P);
   if (!ti.live || ti.qlen <= 0) return;
   const int rows_valid = min(g.query_tile, ti.qoff < ti.qlen ? ti.qlen - ti.qoff : 0) * g.group;
   const int length = ti.recent_begin - ti.sink_len;
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(32 * MAXW, MINB) history_attention_kernel(Hist
       int64_t total = 0;
       const int nt = min(P.task_count[0], P.num_tasks);
       for (int t2 = lane; t2 < nt; t2 += 32) {
-        const TaskInfo tj = load_task(t2, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+        const TaskInfo tj = load_history_task(t2, P);
         if (tj.live && tj.qlen > 0) total += max(0, tj.recent_begin - tj.sink_len);
       }
 #pragma unroll
@@ -467,6 +468,10 @@ struct RawParams {
   oscar_geometry geo;
   float scale_log2;
   int32_t ntiles;
+  // shared-prefix step: split slots [shared_base, shared_base + shared_slots) belong to the
+  // group's partials, of which request r has shared_used[r]; the others are marked empty here
+  const int32_t *shared_used;
+  int32_t shared_base, shared_slots;
 };
 
 constexpr int kRawWarps = 4;
@@ -660,6 +665,9 @@ __global__ void __launch_bounds__(32 * kRawWarps) raw_attention_kernel(RawParams
       dst[16 * mv + gi + 8] = o[mv][2 + r] * inv;
     }
     if (gi == 0) P.lse[orow] = any ? (M[r] * 0.69314718055994531f + logf(L[r])) : -INFINITY;
+    if (P.shared_used)
+      for (int s = P.shared_used[ti.req] + gi; s < P.shared_slots; s += 8)
+        P.lse[orow - P.split_index + P.shared_base + s] = -INFINITY;
   }
 }
 
@@ -762,6 +770,10 @@ constexpr int kFinLive = 4;
 constexpr int kFinThreads = 128;
 constexpr int kFinSmem = (kFinRows * kDim + 2 * kBStageElems) * 2 + 2 * kFinRows * 4;
 
+// HILO (shared-prefix steps): the merged row enters the rotation as bf16 hi + lo parts, lo
+// in the tile row 8 below (an MMA lane holds both rows' sums), and the rotated row is not
+// rounded again: the output is rounded once.  Without it the roundings are the reference's.
+template <bool HILO>
 __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __nv_bfloat16 *sA = reinterpret_cast<__nv_bfloat16 *>(smem_raw);
@@ -773,7 +785,8 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
   const int32_t active = P.counts[1];
   // zero tile rows 8..15 (16 bytes per thread)
   for (int i = threadIdx.x; i < (kFinRows - kFinLive) * kDim / 8; i += kFinThreads)
-    reinterpret_cast<uint4 *>(sA + kFinLive * kDim)[i] = make_uint4(0, 0, 0, 0);
+    if (!HILO || (i * 8 / kDim + kFinLive) % 8 >= kFinLive)
+      reinterpret_cast<uint4 *>(sA + kFinLive * kDim)[i] = make_uint4(0, 0, 0, 0);
   constexpr int RW = kFinLive / 4;  // rows per warp
   float m[RW], w0[RW], w1[RW], den[RW];
   bool valid[RW];
@@ -842,6 +855,15 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
     o.z = pack_bf162(macc[i][4] * inv, macc[i][5] * inv);
     o.w = pack_bf162(macc[i][6] * inv, macc[i][7] * inv);
     *reinterpret_cast<uint4 *>(sA + r * kDim + ((lane ^ (r & 7)) << 3)) = o;
+    if (HILO) {
+      const uint32_t hi[4] = {o.x, o.y, o.z, o.w};
+      uint32_t lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        lo[e] = pack_bf162(macc[i][2 * e] * inv - bf16_bits_to_float(hi[e] & 0xffffu),
+                           macc[i][2 * e + 1] * inv - bf16_bits_to_float(hi[e] >> 16));
+      *reinterpret_cast<uint4 *>(sA + (r + 8) * kDim + ((lane ^ (r & 7)) << 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
     if (lane == 0) {
       s_la[r] = den[i] > 0.f ? m[i] + logf(fmaxf(den[i], 1e-30f)) : -INFINITY;
       s_lb[r] = valid[i] ? P.lse[row * P.split_slots + P.splits] : -INFINITY;
@@ -866,8 +888,8 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
     for (int nj = 0; nj < 8; ++nj) {
       const int col = wn * 64 + nj * 8 + 2 * t;
       // hout is rounded to bf16 (the reference rotate writes bf16)
-      const float h0 = round_bf16(acc[0][nj][2 * hb]);
-      const float h1 = round_bf16(acc[0][nj][2 * hb + 1]);
+      const float h0 = HILO ? acc[0][nj][0] + acc[0][nj][2] : round_bf16(acc[0][nj][2 * hb]);
+      const float h1 = HILO ? acc[0][nj][1] + acc[0][nj][3] : round_bf16(acc[0][nj][2 * hb + 1]);
       float b0 = 0.f, b1 = 0.f;
       if (wb != 0.f) {
         const float2 bb = *reinterpret_cast<const float2 *>(braw + col);
@@ -977,7 +999,7 @@ static int launch_history(const HistParams &P, dim3 grid, size_t smem, cudaStrea
 // consecutive 16-token m-tiles of every chunk; a chunk is all heads of
 // 16 * NM * warps_per_unit tokens (at most one 128-token kernel block).
 // SM count of the current device (cached per device).
-static int sm_count() {
+int sm_count() {
   static int cache[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
@@ -1222,14 +1244,21 @@ extern "C" int oscar_store_windows(const void *key, int64_t ks0, int64_t ks1, co
   return OSCAR_OK;
 }
 
-extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key,
-                                      int64_t ks0, int64_t ks1, const void *value, int64_t vs0, int64_t vs1,
-                                      const uint8_t *history, void *window, const int32_t *qstarts,
-                                      const int32_t *seq_lens, const int32_t *table, const int32_t *counts,
-                                      const int32_t *tasks, const int32_t *task_count, int32_t num_tasks, int64_t n,
-                                      const void *rv, float *scratch_partials, float *scratch_lse, void *output,
-                                      oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
-                                      int32_t *status, void *stream) {
+// The decode step.  `shared`: the plan of a step whose requests share prefixes (its launch
+// fields besides plan, capacities, split count and page count are filled in here), or null.
+struct SharedStep {
+  const int32_t *plan;
+  int32_t max_reqs, items, splits;
+  int64_t num_pages;
+};
+
+static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key, int64_t ks0,
+                       int64_t ks1, const void *value, int64_t vs0, int64_t vs1, const uint8_t *history, void *window,
+                       const int32_t *qstarts, const int32_t *seq_lens, const int32_t *table, const int32_t *counts,
+                       const int32_t *tasks, const int32_t *task_count, int32_t num_tasks, int64_t n, const void *rv,
+                       float *scratch_partials, float *scratch_lse, void *output, oscar_geometry geo, float scale,
+                       int32_t splits, int32_t window_programs, int32_t *status, void *stream,
+                       const SharedStep *shared) {
   if (!paged_geometry_ok(geo) || splits <= 0 || splits > 64 || num_tasks < 0 || n < 0 || window_programs < 0)
     return OSCAR_ERR_INVALID;  // the fused merge holds at most 64 split LSEs per row in one warp
   if (n == 0) return OSCAR_OK;
@@ -1243,6 +1272,9 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
   if (qs0 % 8 || qs1 % 8 || ks0 % 8 || ks1 % 8 || vs0 % 8 || vs1 % 8) return OSCAR_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)stream;
   const int hq = geo.kv_heads * geo.group;
+  const int shared_splits = shared ? shared->splits : 0, all_splits = splits + shared_splits;
+  if (all_splits > 64) return OSCAR_ERR_INVALID;
+  const int32_t *shared_end = shared ? shared->plan + kSharedHead : nullptr;
   bool window_done = false;
   if (num_tasks > 0) {
     HistParams H{};
@@ -1251,7 +1283,8 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
     H.history = history;
     H.qstarts = qstarts, H.seq_lens = seq_lens, H.table = table, H.counts = counts;
     H.tasks = tasks, H.task_count = task_count, H.num_tasks = num_tasks;
-    H.partials = scratch_partials, H.lse = scratch_lse, H.split_slots = splits + 1, H.splits = splits;
+    H.partials = scratch_partials, H.lse = scratch_lse, H.split_slots = all_splits + 1, H.splits = splits;
+    H.shared_end = shared_end;
     H.geo = geo;
     H.scale_log2 = scale * kLog2e;
     H.balanced = 1;
@@ -1267,7 +1300,23 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
       if (cudaEventRecord(side->fork, st) != cudaSuccess || cudaStreamWaitEvent(side->stream, side->fork, 0) != cudaSuccess)
         return OSCAR_ERR_LAUNCH;
     }
-    int rc = history_launch(H, num_tasks, st, side ? side->priority : 0);
+    int rc;
+    if (shared) {
+      // the shared prefix takes the history's place on the caller's stream, and what the
+      // requests have for themselves runs beside it
+      SharedLaunch L{};
+      L.query = reinterpret_cast<const __nv_bfloat16 *>(qrot);
+      L.history = history, L.num_pages = shared->num_pages;
+      L.table = table, L.plan = shared->plan, L.max_reqs = shared->max_reqs, L.items = shared->items;
+      L.partials = scratch_partials, L.lse = scratch_lse, L.split_slots = all_splits + 1, L.slot_base = splits;
+      L.geo = geo;
+      L.scale_log2 = scale * kLog2e;
+      L.status = status;
+      rc = shared_prefix_launch(L, st, side ? side->priority : 0);
+      if (rc == OSCAR_OK) rc = history_launch(H, num_tasks, side ? side->stream : st);
+    } else {
+      rc = history_launch(H, num_tasks, st, side ? side->priority : 0);
+    }
     if (rc) return rc;
     RawParams R{};
     R.query = reinterpret_cast<const __nv_bfloat16 *>(query);
@@ -1278,7 +1327,9 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
     R.window = reinterpret_cast<const __nv_bfloat16 *>(window);
     R.qstarts = qstarts, R.seq_lens = seq_lens, R.table = table, R.counts = counts;
     R.tasks = tasks, R.task_count = task_count;
-    R.partials = scratch_partials, R.lse = scratch_lse, R.split_slots = splits + 1, R.split_index = splits;
+    R.partials = scratch_partials, R.lse = scratch_lse, R.split_slots = all_splits + 1, R.split_index = all_splits;
+    if (shared) R.shared_used = shared_end + shared_up4(shared->max_reqs);
+    R.shared_base = splits, R.shared_slots = shared_splits;
     R.geo = geo;
     R.scale_log2 = scale * kLog2e;
     R.ntiles = (geo.query_tile * geo.group + 7) / 8;
@@ -1296,13 +1347,18 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
                  cudaStreamWaitEvent(st, side->join, 0) != cudaSuccess))
       return OSCAR_ERR_LAUNCH;
   }
-  if (!ensure_dynamic_smem<finalize_kernel>(kFinSmem)) return OSCAR_ERR_LAUNCH;
+  if (!ensure_dynamic_smem<finalize_kernel<false>>(kFinSmem) || !ensure_dynamic_smem<finalize_kernel<true>>(kFinSmem))
+    return OSCAR_ERR_LAUNCH;
   FinalParams F{};
-  F.partials = scratch_partials, F.lse = scratch_lse, F.split_slots = splits + 1, F.splits = splits;
+  F.partials = scratch_partials, F.lse = scratch_lse, F.split_slots = all_splits + 1, F.splits = all_splits;
   F.rows = n * hq, F.hq = hq, F.counts = counts;
   F.rv = reinterpret_cast<const __nv_bfloat16 *>(rv);
   F.out = reinterpret_cast<__nv_bfloat16 *>(output);
-  finalize_kernel<<<(unsigned)((F.rows + kFinLive - 1) / kFinLive), kFinThreads, kFinSmem, st>>>(F);
+  const unsigned fin_blocks = (unsigned)((F.rows + kFinLive - 1) / kFinLive);
+  if (shared)
+    finalize_kernel<true><<<fin_blocks, kFinThreads, kFinSmem, st>>>(F);
+  else
+    finalize_kernel<false><<<fin_blocks, kFinThreads, kFinSmem, st>>>(F);
   OSCAR_CHECK_LAUNCH();
   if (window_programs > 0 && !window_done) {
     window_store_kernel<<<window_programs, 256, 0, st>>>(
@@ -1311,6 +1367,38 @@ extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64
     OSCAR_CHECK_LAUNCH();
   }
   return OSCAR_OK;
+}
+
+extern "C" int oscar_decode_attention(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key,
+                                      int64_t ks0, int64_t ks1, const void *value, int64_t vs0, int64_t vs1,
+                                      const uint8_t *history, void *window, const int32_t *qstarts,
+                                      const int32_t *seq_lens, const int32_t *table, const int32_t *counts,
+                                      const int32_t *tasks, const int32_t *task_count, int32_t num_tasks, int64_t n,
+                                      const void *rv, float *scratch_partials, float *scratch_lse, void *output,
+                                      oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
+                                      int32_t *status, void *stream) {
+  return decode_step(qrot, query, qs0, qs1, key, ks0, ks1, value, vs0, vs1, history, window, qstarts, seq_lens, table,
+                     counts, tasks, task_count, num_tasks, n, rv, scratch_partials, scratch_lse, output, geo, scale,
+                     splits, window_programs, status, stream, nullptr);
+}
+
+extern "C" int oscar_decode_attention_shared(const void *qrot, const void *query, int64_t qs0, int64_t qs1,
+                                             const void *key, int64_t ks0, int64_t ks1, const void *value, int64_t vs0,
+                                             int64_t vs1, const uint8_t *history, int64_t num_pages, void *window,
+                                             const int32_t *qstarts, const int32_t *seq_lens, const int32_t *table,
+                                             const int32_t *counts, const int32_t *tasks, const int32_t *task_count,
+                                             int32_t num_tasks, int64_t n, const void *rv, const int32_t *plan,
+                                             int32_t plan_reqs, int32_t plan_items, int32_t plan_splits,
+                                             float *scratch_partials, float *scratch_lse, void *output,
+                                             oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
+                                             int32_t *status, void *stream) {
+  if (!plan || plan_reqs < 1 || plan_items < 1 || plan_splits < 1 || plan_splits > 63 || num_pages < 1 ||
+      num_pages > INT32_MAX || !(scale > 0.f))
+    return OSCAR_ERR_INVALID;
+  const SharedStep shared{plan, plan_reqs, plan_items, plan_splits, num_pages};
+  return decode_step(qrot, query, qs0, qs1, key, ks0, ks1, value, vs0, vs1, history, window, qstarts, seq_lens, table,
+                     counts, tasks, task_count, num_tasks, n, rv, scratch_partials, scratch_lse, output, geo, scale,
+                     splits, window_programs, status, stream, &shared);
 }
 
 // Test hook, no counterpart in the reference: CTA (0, 0, 0) of every later history launch

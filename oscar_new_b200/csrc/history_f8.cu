@@ -200,7 +200,7 @@ OSCAR_DEVINL F8Item f8_item(const F8Params &T, const F8Small &S, int j, int HG) 
     it.split = (j / T.nhg) % P.splits;
     it.hgrp = j % T.nhg;
   }
-  it.ti = load_task(task, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+  it.ti = load_history_task(task, P);
   const TaskInfo &ti = it.ti;
   if (!ti.live || ti.qlen <= 0) return it;  // rows = 0, nblk = 0: nothing to write
   it.rows = min(g.query_tile, ti.qoff < ti.qlen ? ti.qlen - ti.qoff : 0) * g.group;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) history_f8_kernel(const __grid_
     if (P.balanced) {
       int64_t total = 0;
       for (int t2 = lane; t2 < nt; t2 += 32) {
-        const TaskInfo tj = load_task(t2, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+        const TaskInfo tj = load_history_task(t2, P);
         if (tj.live && tj.qlen > 0) total += max(0, tj.recent_begin - tj.sink_len);
       }
 #pragma unroll
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) history_f8_kernel(const __grid_
         const int t2 = base + lane;
         int cnt = 0, per = 0;
         if (t2 < nt) {
-          const TaskInfo tj = load_task(t2, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+          const TaskInfo tj = load_history_task(t2, P);
           cnt = balanced_splits(tj, span, P.splits, &per) * T.nhg;
         }
         int incl = cnt;
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) history_f8_kernel(const __grid_
       for (int u = blockIdx.x; u < nt * P.splits; u += step) {
         const int t2 = u / P.splits, sp = u % P.splits;
         if (sp * T.nhg < S.pref[t2 + 1] - S.pref[t2]) continue;
-        const TaskInfo tj = load_task(t2, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+        const TaskInfo tj = load_history_task(t2, P);
         if (!tj.live || tj.qlen <= 0) continue;
         const int rows = min(g.query_tile, tj.qoff < tj.qlen ? tj.qlen - tj.qoff : 0) * g.group;
         for (int i = lane; i < g.kv_heads * rows; i += 32) {

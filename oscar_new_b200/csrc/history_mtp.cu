@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kMtpThreads, 1) history_mtp_kernel(HistParams 
   const int task = blockIdx.x, split = blockIdx.y;
   const int h0 = blockIdx.z * P.heads_per_cta;
   const int head = h0 + hl;
-  const TaskInfo ti = load_task(task, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+  const TaskInfo ti = load_history_task(task, P);
   if (!ti.live || ti.qlen <= 0) return;
   const int rows_valid = min(g.query_tile, ti.qoff < ti.qlen ? ti.qlen - ti.qoff : 0) * g.group;
   const int length = ti.recent_begin - ti.sink_len;
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kMtpThreads, 1) history_mtp_kernel(HistParams 
       int64_t total = 0;
       const int nt = min(P.task_count[0], P.num_tasks);
       for (int t2 = lane; t2 < nt; t2 += 32) {
-        const TaskInfo tj = load_task(t2, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, g);
+        const TaskInfo tj = load_history_task(t2, P);
         if (tj.live && tj.qlen > 0) total += max(0, tj.recent_begin - tj.sink_len);
       }
 #pragma unroll

@@ -527,7 +527,8 @@ def dequant_inverse_rotate(history, slots, rk, rv, layout):
 
 
 class DecodeScratch:
-    """Caller-owned split scratch: fp32 partials [n, Hq, splits+1, 256] and lse."""
+    """Caller-owned split scratch: fp32 partials [n, Hq, splits+1, 256] and lse.  A step
+    with a shared prefix takes ``splits`` = its own splits + the plan's."""
 
     def __init__(self, max_tokens: int, hq: int, splits: int, device):
         self.splits = splits
@@ -535,22 +536,100 @@ class DecodeScratch:
         self.lse = torch.empty((max_tokens, hq, splits + 1), dtype=torch.float32, device=device)
 
 
+class SharedPrefix:
+    """Device plan of steps whose requests share prefixes (``prepare_shared_prefix``): for
+    steps of at most ``max_reqs`` requests and ``max_tokens`` tokens.  ``splits``: most parts
+    a group's history is cut into; the default fills the GPU for one group while the split
+    scratch stays under ``scratch_bytes``."""
+
+    def __init__(self, max_reqs: int, max_tokens: int, hq: int, layout, device, splits: int | None = None,
+                 scratch_bytes: int = 256 << 20):
+        if splits is None:
+            fit = scratch_bytes // max(max_tokens * hq * 256 * 4, 1)
+            splits = max(1, min(48, -(-148 // layout.kv_heads), fit))
+        if not 1 <= splits <= 63:
+            raise ValueError("a shared prefix is cut into 1 to 63 splits")
+        sizes = (C.c_int64 * 2)()
+        _lib.call("oscar_shared_prefix_layout", max_reqs, max_tokens, hq, layout.kv_heads, C.addressof(sizes))
+        self.max_reqs, self.items, self.splits, self.hq = max_reqs, int(sizes[0]), splits, hq
+        self.plan = torch.empty(int(sizes[1]), dtype=torch.int32, device=device)
+
+
+def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
+    """Plan one step of requests that share prefixes; once per step, for all its layers.
+
+    groups, prefix_lens: int32 device tensors [requests].  Consecutive requests with the
+    same label >= 0 form a group whose first ``prefix_lens`` tokens (the shortest counts)
+    hold the same history, as after ``fork_requests``; -1: not in a group.  ``shared`` is a
+    ``SharedPrefix`` to fill again (needed for graph capture of changing steps), else a new
+    one.  Returns it, for ``decode_attention(..., shared=)``."""
+    for t, name in ((groups, "groups"), (prefix_lens, "prefix_lens")):
+        if t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] < meta.num_reqs:
+            raise ValueError(f"{name} must be int32 with an entry per request")
+    reqs = min(groups.shape[0], prefix_lens.shape[0], meta.max_num_reqs)
+    if shared is None:
+        tokens = getattr(meta, "num_actual_tokens", None) or meta.num_reqs * max(1, meta.max_query_len)
+        shared = SharedPrefix(reqs, tokens, hq, layout, groups.device)
+    elif shared.hq != hq or shared.max_reqs < meta.num_reqs:
+        raise ValueError("the plan was made for other heads or fewer requests")
+    if reqs < shared.max_reqs:
+        raise ValueError(f"groups and prefix_lens must have the plan's {shared.max_reqs} entries")
+    device = _same_device(groups, prefix_lens, shared.plan, meta.counts)
+    groups, prefix_lens = groups.contiguous(), prefix_lens.contiguous()
+    with device:
+        _lib.call("oscar_prepare_shared_prefix", meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
+                  meta.counts.data_ptr(), groups.data_ptr(), prefix_lens.data_ptr(), shared.max_reqs, shared.items,
+                  shared.splits, geometry(layout, hq, meta.block_tables.stride(0)), shared.plan.data_ptr(),
+                  _stream(groups))
+    return shared
+
+
 def decode_attention(qrot, query, key, value, history, window, meta, layout, scale, splits, rv, output, scratch=None,
-                     store_window=True):
+                     store_window=True, shared=None):
     """History + raw attention, split merge, inverse V rotation, path merge and the
-    window store of one decode / MTP-verify step (reference backend.py:195-226)."""
-    _require_cuda(qrot, query, key, value, history, window, rv, output)
+    window store of one decode / MTP-verify step (reference backend.py:195-226).
+
+    ``shared`` (``prepare_shared_prefix``): the history that groups of requests share is
+    attended once per group, and only the rest per request; ``splits`` is then at most
+    64 - shared.splits (more is cut to that)."""
+    if shared is not None:
+        if shared.hq != query.shape[1] or shared.max_reqs < meta.num_reqs:
+            raise ValueError("the plan was made for other heads or fewer requests")
+        if not scale > 0:
+            raise ValueError("a shared prefix needs a positive softmax scale")
+        if history.numel() % layout.stripe_page_bytes or not history.is_contiguous():
+            raise ValueError("the history view must be whole contiguous pages")
+        if output.dtype != torch.bfloat16 or not output.is_contiguous() or output.numel() != query.numel():
+            raise ValueError("output must be contiguous bf16 [n, Hq * 256]")
+        splits = min(int(splits), 64 - shared.splits)
+        device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan)
+    else:
+        _require_cuda(qrot, query, key, value, history, window, rv, output)
     n, hq, _ = query.shape
     if n == 0:
         return output
-    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != splits:
-        scratch = DecodeScratch(n, hq, splits, query.device)
+    slots = splits + (shared.splits if shared is not None else 0)
+    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != slots:
+        scratch = DecodeScratch(n, hq, slots, query.device)
     query, key, value = _rows(query), _rows(key), _rows(value)
     qrot = qrot.contiguous()
     rv = rv.contiguous()
     geo = _meta_common(meta, layout, hq)
     programs = min(attention_programs(n, meta.max_num_reqs, layout.config.queries_per_tile), meta.tasks.shape[0])
     window_programs = min(n, meta.max_num_reqs) if store_window else 0
+    if shared is not None:
+        with device:
+            _lib.call("oscar_decode_attention_shared", qrot.data_ptr(), query.data_ptr(), query.stride(0),
+                      query.stride(1), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                      value.stride(1), history.data_ptr(), history.numel() // layout.stripe_page_bytes,
+                      window.data_ptr(), meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
+                      meta.block_tables.data_ptr(), meta.counts.data_ptr(), meta.tasks.data_ptr(),
+                      meta.task_count.data_ptr(), programs, n, rv.data_ptr(), shared.plan.data_ptr(), shared.max_reqs,
+                      shared.items, shared.splits, scratch.partials.data_ptr(), scratch.lse.data_ptr(),
+                      output.data_ptr(), geo, float(scale), int(splits), window_programs, _status(query),
+                      _stream(query))
+        _checked("oscar_decode_attention_shared", query)
+        return output
     _lib.call("oscar_decode_attention", qrot.data_ptr(), query.data_ptr(), query.stride(0), query.stride(1),
               key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
               history.data_ptr(), window.data_ptr(), meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
