@@ -120,4 +120,6 @@ def check(status: int, name: str):
 
 
 def call(name: str, *args):
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status:
+        check(status, name)

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(32 * MAXW, MINB) history_attention_kernel(Hist
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       if (lane == 0) {
         const int64_t span = (total * gridDim.z + P.target_ctas - 1) / max(P.target_ctas, 1);
-        s_span = (int)(span < kMinSplitTokens ? (int64_t)kMinSplitTokens : (span > (1 << 30) ? (int64_t)(1 << 30) : span));
+        s_span = (int)(span < P.min_split ? (int64_t)P.min_split : (span > (1 << 30) ? (int64_t)(1 << 30) : span));
       }
     }
     __syncthreads();
@@ -474,8 +474,10 @@ struct RawParams {
   int32_t shared_base, shared_slots;
 };
 
-constexpr int kRawWarps = 4;
-constexpr int kRawSmem = kRawWarps * 2 * 16 * kDim * 2;  // per warp K and V 16-token tiles
+// Warps per CTA: 4 (three CTAs per SM), or 12 for the few CTAs of a small shared-prefix step,
+// whose tokens then pass in a third of the steps (4 requests x 321 tokens, one KV head).
+constexpr int kRawWarps = 4, kRawWideWarps = 12;
+constexpr int raw_smem(int warps) { return warps * 2 * 16 * kDim * 2; }  // per warp K and V 16-token tiles
 
 OSCAR_DEVINL const __nv_bfloat16 *raw_token_row(const RawParams &P, const TaskInfo &ti, int64_t owner,
                                                 int idx, int kv, int head) {
@@ -491,7 +493,8 @@ OSCAR_DEVINL const __nv_bfloat16 *raw_token_row(const RawParams &P, const TaskIn
                  : P.value + (int64_t)cur * P.vs0 + (int64_t)head * P.vs1;
 }
 
-__global__ void __launch_bounds__(32 * kRawWarps) raw_attention_kernel(RawParams P) {
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) raw_attention_kernel(RawParams P) {
   extern __shared__ __align__(128) uint8_t smem[];
   const oscar_geometry &g = P.geo;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -530,18 +533,21 @@ __global__ void __launch_bounds__(32 * kRawWarps) raw_attention_kernel(RawParams
   for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
 #pragma unroll 1
-  for (int base = 16 * warp; base < total; base += 16 * kRawWarps) {
-    // stage 16 K and V rows (swizzled 16-byte chunks)
+  for (int base = 16 * warp; base < total; base += 16 * WARPS) {
+    // stage 16 K and V rows (swizzled 16-byte chunks); lanes 0-15 find the rows of K, 16-31 of V
+    const int own = base + (lane & 15);
+    const uint64_t row_of = own < total ? reinterpret_cast<uint64_t>(raw_token_row(P, ti, owner, own, lane >> 4, head)) : 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int c = lane + 32 * i;  // 16 rows x 32 chunks
-      const int r = c >> 5, ch = c & 31;
+      const int r = i, ch = lane;  // 16 rows x 32 chunks
       const int idx = base + r;
+      const auto *krow = reinterpret_cast<const __nv_bfloat16 *>(__shfl_sync(0xffffffffu, row_of, i));
+      const auto *vrow = reinterpret_cast<const __nv_bfloat16 *>(__shfl_sync(0xffffffffu, row_of, 16 + i));
       __nv_bfloat16 *dk = sk + r * kDim + ((ch ^ (r & 7)) << 3);
       __nv_bfloat16 *dv = sv + r * kDim + ((ch ^ (r & 7)) << 3);
       if (idx < total) {
-        cp_async_16(smem_u32(dk), raw_token_row(P, ti, owner, idx, 0, head) + ch * 8);
-        cp_async_16(smem_u32(dv), raw_token_row(P, ti, owner, idx, 1, head) + ch * 8);
+        cp_async_16(smem_u32(dk), krow + ch * 8);
+        cp_async_16(smem_u32(dv), vrow + ch * 8);
       } else {
         *reinterpret_cast<uint4 *>(dk) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4 *>(dv) = make_uint4(0, 0, 0, 0);
@@ -624,50 +630,55 @@ __global__ void __launch_bounds__(32 * kRawWarps) raw_attention_kernel(RawParams
   rec[66 * 32 + lane] = l_run[0];
   rec[67 * 32 + lane] = l_run[1];
   __syncthreads();
-  if (warp != 0) return;
+  // every warp merges and writes its share of the dims, the warps' records in order
   float M[2] = {-INFINITY, -INFINITY};
-  for (int w = 0; w < kRawWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     M[0] = fmaxf(M[0], xch[w * 68 * 32 + 64 * 32 + lane]);
     M[1] = fmaxf(M[1], xch[w * 68 * 32 + 65 * 32 + lane]);
   }
   float L[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  for (int w = 0; w < kRawWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     const float *rw = xch + w * 68 * 32;
     const float mw0 = rw[64 * 32 + lane], mw1 = rw[65 * 32 + lane];
-    const float e0 = mw0 == -INFINITY ? 0.f : ex2(mw0 - M[0]);
-    const float e1 = mw1 == -INFINITY ? 0.f : ex2(mw1 - M[1]);
-    L[0] = fmaf(e0, rw[66 * 32 + lane], L[0]);
-    L[1] = fmaf(e1, rw[67 * 32 + lane], L[1]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      o[i][0] = fmaf(e0, rw[(i * 4 + 0) * 32 + lane], o[i][0]);
-      o[i][1] = fmaf(e1, rw[(i * 4 + 1) * 32 + lane], o[i][1]);
-      o[i][2] = fmaf(e0, rw[(i * 4 + 2) * 32 + lane], o[i][2]);
-      o[i][3] = fmaf(e1, rw[(i * 4 + 3) * 32 + lane], o[i][3]);
-    }
+    L[0] = fmaf(mw0 == -INFINITY ? 0.f : ex2(mw0 - M[0]), rw[66 * 32 + lane], L[0]);
+    L[1] = fmaf(mw1 == -INFINITY ? 0.f : ex2(mw1 - M[1]), rw[67 * 32 + lane], L[1]);
   }
+  const float inv[2] = {L[0] > 0.f ? 1.0f / L[0] : 0.f, L[1] > 0.f ? 1.0f / L[1] : 0.f};
+  int64_t orow[2];
+  bool live[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int row = 8 * ntile + 2 * t + r;
-    if (row >= rows_valid) continue;
+    live[r] = row < rows_valid;
     const int tok = ti.qstart + ti.qoff + row / g.group;
     const int qh = head * g.group + row % g.group;
-    const int64_t orow = ((int64_t)tok * g.kv_heads * g.group + qh) * P.split_slots + P.split_index;
-    const bool any = L[r] > 0.f;
-    const float inv = any ? 1.0f / L[r] : 0.f;
-    float *dst = P.partials + orow * kDim;
-    // O^T fragment: m-tile mv rows (dims) 16mv + gi and 16mv + gi + 8
-#pragma unroll
-    for (int mv = 0; mv < 16; ++mv) {
-      dst[16 * mv + gi] = o[mv][r] * inv;
-      dst[16 * mv + gi + 8] = o[mv][2 + r] * inv;
-    }
-    if (gi == 0) P.lse[orow] = any ? (M[r] * 0.69314718055994531f + logf(L[r])) : -INFINITY;
+    orow[r] = ((int64_t)tok * g.kv_heads * g.group + qh) * P.split_slots + P.split_index;
+    if (!live[r] || warp != 0) continue;
+    if (gi == 0) P.lse[orow[r]] = L[r] > 0.f ? (M[r] * 0.69314718055994531f + logf(L[r])) : -INFINITY;
     if (P.shared_used)
       for (int s = P.shared_used[ti.req] + gi; s < P.shared_slots; s += 8)
-        P.lse[orow - P.split_index + P.shared_base + s] = -INFINITY;
+        P.lse[orow[r] - P.split_index + P.shared_base + s] = -INFINITY;
+  }
+  // O^T fragment: m-tile mv rows (dims) 16mv + gi and 16mv + gi + 8
+  for (int mv = warp; mv < 16; mv += WARPS) {
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < WARPS; ++w) {
+      const float *rw = xch + w * 68 * 32;
+      const float mw0 = rw[64 * 32 + lane], mw1 = rw[65 * 32 + lane];
+      const float e0 = mw0 == -INFINITY ? 0.f : ex2(mw0 - M[0]);
+      const float e1 = mw1 == -INFINITY ? 0.f : ex2(mw1 - M[1]);
+      a[0] = fmaf(e0, rw[(mv * 4 + 0) * 32 + lane], a[0]);
+      a[1] = fmaf(e1, rw[(mv * 4 + 1) * 32 + lane], a[1]);
+      a[2] = fmaf(e0, rw[(mv * 4 + 2) * 32 + lane], a[2]);
+      a[3] = fmaf(e1, rw[(mv * 4 + 3) * 32 + lane], a[3]);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      if (!live[r]) continue;
+      float *dst = P.partials + orow[r] * kDim;
+      dst[16 * mv + gi] = a[r] * inv[r];
+      dst[16 * mv + gi + 8] = a[2 + r] * inv[r];
+    }
   }
 }
 
@@ -770,10 +781,6 @@ constexpr int kFinLive = 4;
 constexpr int kFinThreads = 128;
 constexpr int kFinSmem = (kFinRows * kDim + 2 * kBStageElems) * 2 + 2 * kFinRows * 4;
 
-// HILO (shared-prefix steps): the merged row enters the rotation as bf16 hi + lo parts, lo
-// in the tile row 8 below (an MMA lane holds both rows' sums), and the rotated row is not
-// rounded again: the output is rounded once.  Without it the roundings are the reference's.
-template <bool HILO>
 __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   __nv_bfloat16 *sA = reinterpret_cast<__nv_bfloat16 *>(smem_raw);
@@ -785,8 +792,7 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
   const int32_t active = P.counts[1];
   // zero tile rows 8..15 (16 bytes per thread)
   for (int i = threadIdx.x; i < (kFinRows - kFinLive) * kDim / 8; i += kFinThreads)
-    if (!HILO || (i * 8 / kDim + kFinLive) % 8 >= kFinLive)
-      reinterpret_cast<uint4 *>(sA + kFinLive * kDim)[i] = make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4 *>(sA + kFinLive * kDim)[i] = make_uint4(0, 0, 0, 0);
   constexpr int RW = kFinLive / 4;  // rows per warp
   float m[RW], w0[RW], w1[RW], den[RW];
   bool valid[RW];
@@ -855,15 +861,6 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
     o.z = pack_bf162(macc[i][4] * inv, macc[i][5] * inv);
     o.w = pack_bf162(macc[i][6] * inv, macc[i][7] * inv);
     *reinterpret_cast<uint4 *>(sA + r * kDim + ((lane ^ (r & 7)) << 3)) = o;
-    if (HILO) {
-      const uint32_t hi[4] = {o.x, o.y, o.z, o.w};
-      uint32_t lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        lo[e] = pack_bf162(macc[i][2 * e] * inv - bf16_bits_to_float(hi[e] & 0xffffu),
-                           macc[i][2 * e + 1] * inv - bf16_bits_to_float(hi[e] >> 16));
-      *reinterpret_cast<uint4 *>(sA + (r + 8) * kDim + ((lane ^ (r & 7)) << 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
     if (lane == 0) {
       s_la[r] = den[i] > 0.f ? m[i] + logf(fmaxf(den[i], 1e-30f)) : -INFINITY;
       s_lb[r] = valid[i] ? P.lse[row * P.split_slots + P.splits] : -INFINITY;
@@ -888,8 +885,8 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
     for (int nj = 0; nj < 8; ++nj) {
       const int col = wn * 64 + nj * 8 + 2 * t;
       // hout is rounded to bf16 (the reference rotate writes bf16)
-      const float h0 = HILO ? acc[0][nj][0] + acc[0][nj][2] : round_bf16(acc[0][nj][2 * hb]);
-      const float h1 = HILO ? acc[0][nj][1] + acc[0][nj][3] : round_bf16(acc[0][nj][2 * hb + 1]);
+      const float h0 = round_bf16(acc[0][nj][2 * hb]);
+      const float h1 = round_bf16(acc[0][nj][2 * hb + 1]);
       float b0 = 0.f, b1 = 0.f;
       if (wb != 0.f) {
         const float2 bb = *reinterpret_cast<const float2 *>(braw + col);
@@ -905,17 +902,11 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
 // window store (reference _window_store_kernel): CTA per request, warp per
 // (window index, head) pair, 16-byte lanes.
 // ----------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) window_store_kernel(const __nv_bfloat16 *__restrict__ key,
-                                                           int64_t ks0, int64_t ks1,
-                                                           const __nv_bfloat16 *__restrict__ value,
-                                                           int64_t vs0, int64_t vs1,
-                                                           __nv_bfloat16 *__restrict__ window,
-                                                           const int32_t *__restrict__ qstarts,
-                                                           const int32_t *__restrict__ seq_lens,
-                                                           const int32_t *__restrict__ table,
-                                                           const int32_t *__restrict__ counts,
-                                                           oscar_geometry g) {
-  const int req = blockIdx.x;
+OSCAR_DEVINL void store_window(int req, int warps, const __nv_bfloat16 *__restrict__ key, int64_t ks0, int64_t ks1,
+                               const __nv_bfloat16 *__restrict__ value, int64_t vs0, int64_t vs1,
+                               __nv_bfloat16 *__restrict__ window, const int32_t *__restrict__ qstarts,
+                               const int32_t *__restrict__ seq_lens, const int32_t *__restrict__ table,
+                               const int32_t *__restrict__ counts, const oscar_geometry &g) {
   if (req >= counts[0]) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int qstart = qstarts[req];
@@ -934,7 +925,7 @@ __global__ void __launch_bounds__(256) window_store_kernel(const __nv_bfloat16 *
   const int ring_lo = max(max(lo, g.sink), seq - g.ring);
   const int n_ring = max(0, seq - ring_lo);
   const int entries = (n_sink + n_ring) * g.kv_heads;
-  for (int e = warp; e < entries; e += 8) {
+  for (int e = warp; e < entries; e += warps) {
     const int k = e / g.kv_heads, head = e % g.kv_heads;
     const int pos = k < n_sink ? lo + k : ring_lo + (k - n_sink);
     const int idx = pos < g.sink ? pos : g.sink + pos % g.ring;
@@ -943,6 +934,160 @@ __global__ void __launch_bounds__(256) window_store_kernel(const __nv_bfloat16 *
     const uint4 kv1 = *reinterpret_cast<const uint4 *>(value + (int64_t)cur * vs0 + (int64_t)head * vs1 + lane * 8);
     *reinterpret_cast<uint4 *>(window + window_elem_offset(owner, idx, 0, head, g) + lane * 8) = kv0;
     *reinterpret_cast<uint4 *>(window + window_elem_offset(owner, idx, 1, head, g) + lane * 8) = kv1;
+  }
+}
+
+__global__ void __launch_bounds__(256) window_store_kernel(const __nv_bfloat16 *__restrict__ key,
+                                                           int64_t ks0, int64_t ks1,
+                                                           const __nv_bfloat16 *__restrict__ value,
+                                                           int64_t vs0, int64_t vs1,
+                                                           __nv_bfloat16 *__restrict__ window,
+                                                           const int32_t *__restrict__ qstarts,
+                                                           const int32_t *__restrict__ seq_lens,
+                                                           const int32_t *__restrict__ table,
+                                                           const int32_t *__restrict__ counts,
+                                                           oscar_geometry g) {
+  store_window(blockIdx.x, 8, key, ks0, ks1, value, vs0, vs1, window, qstarts, seq_lens, table, counts, g);
+}
+
+// ----------------------------------------------------------------------------
+// the same epilogue of a step with shared prefixes: one warp per row, 16 rows per CTA (one
+// wave up to 2368 rows).  All of Rv^T is on its way to shared memory while the splits are
+// merged, and only the splits with weight are read, eight at a time.  The merged row enters
+// the rotation as bf16 hi + lo parts (two tiles of the MMA) and the rotated row is not
+// rounded again: the output is rounded once.  Blocks behind the rows' store the windows (the
+// raw path that reads them is done), one request each.
+// ----------------------------------------------------------------------------
+constexpr int kFinWideRows = 16;
+constexpr int kFinWideThreads = 32 * kFinWideRows;
+constexpr int kFinWideSmem = (kDim * kDim + 2 * kFinWideRows * kDim) * 2 + 2 * kFinWideRows * 4;
+
+struct WindowParams {
+  const __nv_bfloat16 *key, *value;
+  int64_t ks0, ks1, vs0, vs1;
+  __nv_bfloat16 *window;
+  const int32_t *qstarts, *seq_lens, *table;
+  oscar_geometry geo;
+};
+
+__global__ void __launch_bounds__(kFinWideThreads, 1) finalize_wide_kernel(FinalParams P, WindowParams W, int row_blocks) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  if (blockIdx.x >= row_blocks) {
+    store_window(blockIdx.x - row_blocks, kFinWideRows, W.key, W.ks0, W.ks1, W.value, W.vs0, W.vs1, W.window, W.qstarts,
+                 W.seq_lens, W.table, P.counts, W.geo);
+    return;
+  }
+  __nv_bfloat16 *sB = reinterpret_cast<__nv_bfloat16 *>(smem_raw);  // [256 n][256 k], chunks ^ (n & 7)
+  __nv_bfloat16 *sA = sB + kDim * kDim;                             // hi rows, then lo rows
+  float *s_la = reinterpret_cast<float *>(sA + 2 * kFinWideRows * kDim), *s_lb = s_la + kFinWideRows;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Rv rows in two halves of k: the first product waits for half of them
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < kDim * 16 / kFinWideThreads; ++i) {
+      const int c = threadIdx.x + i * kFinWideThreads, n = c >> 4, ch = 16 * h + (c & 15);
+      cp_async_16(smem_u32(sB + n * kDim + ((ch ^ (n & 7)) << 3)), P.rv + n * kDim + ch * 8);
+    }
+    cp_async_commit();
+  }
+  const int64_t row0 = (int64_t)blockIdx.x * kFinWideRows, row = row0 + warp;
+  const bool valid = row < P.rows && row / P.hq < P.counts[1];
+  const float *lrow = P.lse + row * P.split_slots;
+  const float l0 = valid && lane < P.splits ? lrow[lane] : -INFINITY;
+  const float l1 = valid && lane + 32 < P.splits ? lrow[lane + 32] : -INFINITY;
+  float top = fmaxf(l0, l1);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float safe = top == -INFINITY ? 0.f : top;
+  const float w0 = expf(l0 - safe), w1 = expf(l1 - safe);
+  float den = w0 + w1;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  // a NaN lse is a split with weight: it reaches the row
+  uint64_t left = (uint64_t)__ballot_sync(0xffffffffu, w0 != 0.f) | (uint64_t)__ballot_sync(0xffffffffu, w1 != 0.f) << 32;
+  const float *src = P.partials + row * P.split_slots * kDim + lane * 8;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  while (left) {
+    float w[8];
+    float4 x[8][2];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int sp = left ? __ffsll((long long)left) - 1 : -1;
+      left &= left - 1;  // 0 stays 0
+      const float wa = __shfl_sync(0xffffffffu, w0, sp & 31), wb = __shfl_sync(0xffffffffu, w1, sp & 31);
+      w[u] = sp < 0 ? 0.f : (sp < 32 ? wa : wb);
+      const float4 *at = reinterpret_cast<const float4 *>(src + (int64_t)max(sp, 0) * kDim);
+      x[u][0] = sp < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : at[0];
+      x[u][1] = sp < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : at[1];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      acc[0] = fmaf(w[u], x[u][0].x, acc[0]), acc[1] = fmaf(w[u], x[u][0].y, acc[1]);
+      acc[2] = fmaf(w[u], x[u][0].z, acc[2]), acc[3] = fmaf(w[u], x[u][0].w, acc[3]);
+      acc[4] = fmaf(w[u], x[u][1].x, acc[4]), acc[5] = fmaf(w[u], x[u][1].y, acc[5]);
+      acc[6] = fmaf(w[u], x[u][1].z, acc[6]), acc[7] = fmaf(w[u], x[u][1].w, acc[7]);
+    }
+  }
+  {
+    const float inv = den != 0.f ? 1.0f / den : 0.f;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;
+      hi[e] = pack_bf162(a, b);
+      lo[e] = pack_bf162(a - bf16_bits_to_float(hi[e] & 0xffffu), b - bf16_bits_to_float(hi[e] >> 16));
+    }
+    const int at = warp * kDim + ((lane ^ (warp & 7)) << 3);
+    *reinterpret_cast<uint4 *>(sA + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(sA + kFinWideRows * kDim + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (lane == 0) {
+      s_la[warp] = den != 0.f ? top + logf(den) : -INFINITY;
+      s_lb[warp] = valid ? lrow[P.splits] : -INFINITY;
+    }
+  }
+  // warp w: columns 16w .. 16w + 15 of all rows
+  float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h == 0)
+      cp_async_wait<1>();
+    else
+      cp_async_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int kk = 8 * h; kk < 8 * h + 8; ++kk) {
+      uint32_t ah[4], al[4], b[4];
+      const int ar = lane & 15, ak = 16 * kk + (lane >> 4) * 8;
+      ldmatrix_x4(ah, smem_u32(sA + a_index(ar, ak)));
+      ldmatrix_x4(al, smem_u32(sA + kFinWideRows * kDim + a_index(ar, ak)));
+      const int n = 16 * warp + (lane >> 4) * 8 + (lane & 7), k = 16 * kk + ((lane >> 3) & 1) * 8;
+      ldmatrix_x4(b, smem_u32(sB + n * kDim + (((k >> 3) ^ (n & 7)) << 3)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mma_bf16_16816(c[j], ah[0], ah[1], ah[2], ah[3], b[2 * j], b[2 * j + 1]);
+        mma_bf16_16816(c[j], al[0], al[1], al[2], al[3], b[2 * j], b[2 * j + 1]);
+      }
+    }
+  }
+  const int gq = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = gq + 8 * half;
+    if (row0 + r >= P.rows) continue;
+    const float xa = s_la[r], xb = s_lb[r];
+    float m = fmaxf(xa, xb);
+    m = m == -INFINITY ? 0.f : m;
+    const float wa = expf(xa - m), wb = expf(xb - m);
+    const float inv = 1.0f / fmaxf(wa + wb, 1e-30f);
+    const float *braw = P.partials + ((row0 + r) * P.split_slots + P.splits) * kDim;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = 16 * warp + 8 * j + 2 * t;
+      const float2 raw = wb != 0.f ? *reinterpret_cast<const float2 *>(braw + col) : make_float2(0.f, 0.f);
+      *reinterpret_cast<uint32_t *>(P.out + (row0 + r) * kDim + col) =
+          pack_bf162((wa * c[j][2 * half] + wb * raw.x) * inv, (wa * c[j][2 * half + 1] + wb * raw.y) * inv);
+    }
   }
 }
 
@@ -1124,12 +1269,19 @@ static RawSide *raw_side(cudaStream_t caller) {
   return c.ok ? &c : nullptr;
 }
 
-static int raw_launch(const RawParams &P, int32_t num_tasks, cudaStream_t stream) {
-  if (!ensure_dynamic_smem<raw_attention_kernel>(kRawSmem)) return OSCAR_ERR_LAUNCH;
-  dim3 grid(num_tasks, P.geo.kv_heads, P.ntiles);
-  raw_attention_kernel<<<grid, 32 * kRawWarps, kRawSmem, stream>>>(P);
+template <int WARPS>
+static int raw_launch_warps(const RawParams &P, dim3 grid, cudaStream_t stream) {
+  if (!ensure_dynamic_smem<raw_attention_kernel<WARPS>>(raw_smem(WARPS))) return OSCAR_ERR_LAUNCH;
+  raw_attention_kernel<WARPS><<<grid, 32 * WARPS, raw_smem(WARPS), stream>>>(P);
   OSCAR_CHECK_LAUNCH();
   return OSCAR_OK;
+}
+
+static int raw_launch(const RawParams &P, int32_t num_tasks, cudaStream_t stream) {
+  dim3 grid(num_tasks, P.geo.kv_heads, P.ntiles);
+  if (P.shared_used && (int64_t)num_tasks * P.geo.kv_heads * P.ntiles <= sm_count())
+    return raw_launch_warps<kRawWideWarps>(P, grid, stream);
+  return raw_launch_warps<kRawWarps>(P, grid, stream);
 }
 
 }  // namespace oscar
@@ -1289,6 +1441,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     H.scale_log2 = scale * kLog2e;
     H.balanced = 1;
     H.target_ctas = 8 * sm_count();
+    H.min_split = shared ? kMinSharedSplit : kMinSplitTokens;
     H.status = status;
     // history on the caller's stream at the greatest priority, the raw path and then the
     // window store beside it on the side stream (joined before the merge); without a side
@@ -1335,7 +1488,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     R.ntiles = (geo.query_tile * geo.group + 7) / 8;
     rc = raw_launch(R, num_tasks, side ? side->stream : st);
     if (rc) return rc;
-    if (side && window_programs > 0) {
+    if (side && window_programs > 0 && !shared) {
       // the window store overwrites ring slots the raw path reads: after it, same stream
       window_store_kernel<<<window_programs, 256, 0, side->stream>>>(
           reinterpret_cast<const __nv_bfloat16 *>(key), ks0, ks1, reinterpret_cast<const __nv_bfloat16 *>(value),
@@ -1347,18 +1500,22 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
                  cudaStreamWaitEvent(st, side->join, 0) != cudaSuccess))
       return OSCAR_ERR_LAUNCH;
   }
-  if (!ensure_dynamic_smem<finalize_kernel<false>>(kFinSmem) || !ensure_dynamic_smem<finalize_kernel<true>>(kFinSmem))
-    return OSCAR_ERR_LAUNCH;
   FinalParams F{};
   F.partials = scratch_partials, F.lse = scratch_lse, F.split_slots = all_splits + 1, F.splits = all_splits;
   F.rows = n * hq, F.hq = hq, F.counts = counts;
   F.rv = reinterpret_cast<const __nv_bfloat16 *>(rv);
   F.out = reinterpret_cast<__nv_bfloat16 *>(output);
-  const unsigned fin_blocks = (unsigned)((F.rows + kFinLive - 1) / kFinLive);
-  if (shared)
-    finalize_kernel<true><<<fin_blocks, kFinThreads, kFinSmem, st>>>(F);
-  else
-    finalize_kernel<false><<<fin_blocks, kFinThreads, kFinSmem, st>>>(F);
+  if (shared) {
+    if (!ensure_dynamic_smem<finalize_wide_kernel>(kFinWideSmem)) return OSCAR_ERR_LAUNCH;
+    const WindowParams W{reinterpret_cast<const __nv_bfloat16 *>(key), reinterpret_cast<const __nv_bfloat16 *>(value),
+                         ks0, ks1, vs0, vs1, reinterpret_cast<__nv_bfloat16 *>(window), qstarts, seq_lens, table, geo};
+    const int row_blocks = (int)((F.rows + kFinWideRows - 1) / kFinWideRows);
+    finalize_wide_kernel<<<row_blocks + window_programs, kFinWideThreads, kFinWideSmem, st>>>(F, W, row_blocks);
+    window_done = true;
+  } else {
+    if (!ensure_dynamic_smem<finalize_kernel>(kFinSmem)) return OSCAR_ERR_LAUNCH;
+    finalize_kernel<<<(unsigned)((F.rows + kFinLive - 1) / kFinLive), kFinThreads, kFinSmem, st>>>(F);
+  }
   OSCAR_CHECK_LAUNCH();
   if (window_programs > 0 && !window_done) {
     window_store_kernel<<<window_programs, 256, 0, st>>>(

@@ -35,10 +35,11 @@ struct HistParams {
   int32_t stage_bytes;
   int32_t *status;        // nullable error word
   // balanced splits (decode path): a request of L history tokens uses
-  // clamp(ceil(L / span), 1, splits) splits, span = max(kMinSplitTokens,
+  // clamp(ceil(L / span), 1, splits) splits, span = max(min_split,
   // total history * head groups / target_ctas); empty splits write only lse = -inf
   int32_t balanced;
   int32_t target_ctas;
+  int32_t min_split;
   // test hook (oscar_test_set_wait_fault): CTA 0 never issues the copy of this chunk / tile
   // (-1: none); every bounded device wait gives up after wait_probes probes
   int32_t withhold;
@@ -49,6 +50,10 @@ struct HistParams {
 };
 
 constexpr int kMinSplitTokens = 1024;
+// In a shared-prefix step a request's own history is short and its splits fill the GPU only
+// when they are: 24 requests of up to 700 own tokens, 4 queries each, take 66 us in
+// 1024-token splits.
+constexpr int kMinSharedSplit = 128;
 
 struct TaskInfo {
   bool live;

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) history_f8_kernel(const __grid_
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       const int64_t span0 = (total * T.nhg + P.target_ctas - 1) / max(P.target_ctas, 1);
-      const int span = (int)(span0 < kMinSplitTokens ? (int64_t)kMinSplitTokens
+      const int span = (int)(span0 < P.min_split ? (int64_t)P.min_split
                                                      : (span0 > (1 << 30) ? (int64_t)(1 << 30) : span0));
       int run = 0;
       for (int base = 0; base < nt; base += 32) {

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kMtpThreads, 1) history_mtp_kernel(HistParams 
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
       if (lane == 0) {
         const int64_t span = (total * gridDim.z + P.target_ctas - 1) / max(P.target_ctas, 1);
-        s_span = (int)(span < kMinSplitTokens ? (int64_t)kMinSplitTokens : (span > (1 << 30) ? (int64_t)(1 << 30) : span));
+        s_span = (int)(span < P.min_split ? (int64_t)P.min_split : (span > (1 << 30) ? (int64_t)(1 << 30) : span));
       }
     }
     __syncthreads();

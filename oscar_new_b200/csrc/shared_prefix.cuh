@@ -8,7 +8,7 @@ namespace oscar {
 
 // Plan (int32 words, device): header, then per request the end of the history that its
 // group's tiles cover (0: none) and the split slots they fill, then the work items.
-constexpr int kSharedHead = 8;  // [0] items
+constexpr int kSharedHead = 8;  // [0] items, [1] CTAs that work on them
 struct SharedItem {
   int32_t tok0;            // first token of the group
   int32_t row0, rows;      // this tile's rows of the group (row i: token i / G, query head i % G)

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -53,7 +54,8 @@ def read_status(device=None, clear: bool = True) -> int:
 
 
 def _status(t: torch.Tensor):
-    return status_word(t.device).data_ptr()
+    word = _STATUS_WORDS.get(t.get_device())
+    return (status_word(t.device) if word is None else word).data_ptr()
 
 
 def _checked(name: str, t: torch.Tensor):
@@ -65,7 +67,8 @@ def _checked(name: str, t: torch.Tensor):
 
 
 def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle of torch.cuda.current_stream(t.device), without building a Stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t):
@@ -254,22 +257,31 @@ def prefill_attention(query, key, value, query_start_loc, num_reqs: int, max_que
     return out
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _dense(t: torch.Tensor):
+    return t if t.is_contiguous() else t.contiguous()
+
+
+
 def _same_device(*tensors):
-    """All on one CUDA device; returns the context that makes it current if it is not."""
-    _require_cuda(*tensors)
-    given = [t for t in tensors if t is not None]
-    device = given[0].device
-    if any(t.device != device for t in given):
-        raise ValueError(f"tensors on several devices: {sorted({str(t.device) for t in given})}")
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    """All on one CUDA device (None: skipped, but not the first); returns the context that
+    makes it current if it is not."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _require_cuda(*tensors)
+            raise ValueError(f"tensors on several devices: {sorted({str(t.device) for t in tensors if t is not None})}")
+    if index < 0:
+        _require_cuda(*tensors)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _output_rows(out, like):
     """``out`` (or a new tensor) as the bf16 rows a kernel writes for ``like``."""
     if out is None:
-        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+        return like.new_empty(like.shape)
     if out.dtype != torch.bfloat16 or out.shape != like.shape:
         raise ValueError(f"expected a bf16 output of shape {tuple(like.shape)}, got {tuple(out.shape)} {out.dtype}")
     if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
@@ -376,7 +388,7 @@ def _pool_list(pool, *lists):
             raise ValueError("row lists are int32 [count], all of one length")
     if lists[0].shape[0] > pool.max_reqs:
         raise ValueError(f"{lists[0].shape[0]} entries for a pool of {pool.max_reqs} rows")
-    return [t.contiguous() for t in lists]
+    return [_dense(t) for t in lists]
 
 
 def fork_requests(pool, parents, children, history, window):
@@ -391,7 +403,7 @@ def fork_requests(pool, parents, children, history, window):
     pool.check_stripes(history, window)
     parents, children = _pool_list(pool, parents, children)
     device = _same_device(pool.arena, parents, children, history, window)
-    result = torch.empty(parents.shape, dtype=torch.int32, device=parents.device)
+    result = parents.new_empty(parents.shape)
     with device:
         _lib.call("oscar_fork_requests", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
                   parents.data_ptr(), children.data_ptr(), parents.shape[0], history.data_ptr(), window.data_ptr(),
@@ -409,7 +421,7 @@ def resize_requests(pool, rows, lens):
     row that an earlier entry names)."""
     rows, lens = _pool_list(pool, rows, lens)
     device = _same_device(pool.arena, rows, lens)
-    result = torch.empty(rows.shape, dtype=torch.int32, device=rows.device)
+    result = rows.new_empty(rows.shape)
     with device:
         _lib.call("oscar_resize_requests", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
                   pool.layout.physical_block_tokens, rows.data_ptr(), lens.data_ptr(), rows.shape[0],
@@ -423,8 +435,7 @@ def compact_pages(pool, history, window):
     pages], moved_to int32 [num_pages]: each page's new number, -1 for a free page)."""
     pool.check_stripes(history, window)
     device = _same_device(pool.arena, history, window)
-    summary = torch.empty(2, dtype=torch.int32, device=pool.device)
-    moved_to = torch.empty(pool.num_pages, dtype=torch.int32, device=pool.device)
+    summary, moved_to = pool.arena.new_empty(2), pool.arena.new_empty(pool.num_pages)
     with device:
         _lib.call("oscar_compact_pages", pool.arena.data_ptr(), pool.num_pages, pool.max_reqs, pool.columns,
                   history.data_ptr(), window.data_ptr(), pool.geometry, summary.data_ptr(), moved_to.data_ptr(),
@@ -536,6 +547,14 @@ class DecodeScratch:
         self.lse = torch.empty((max_tokens, hq, splits + 1), dtype=torch.float32, device=device)
 
 
+@functools.lru_cache(maxsize=256)
+def _shared_sizes(max_reqs: int, max_tokens: int, hq: int, kv_heads: int):
+    """(work items, int32 words) of a shared-prefix plan (host-only call, no device)."""
+    sizes = (C.c_int64 * 2)()
+    _lib.call("oscar_shared_prefix_layout", max_reqs, max_tokens, hq, kv_heads, C.addressof(sizes))
+    return int(sizes[0]), int(sizes[1])
+
+
 class SharedPrefix:
     """Device plan of steps whose requests share prefixes (``prepare_shared_prefix``): for
     steps of at most ``max_reqs`` requests and ``max_tokens`` tokens.  ``splits``: most parts
@@ -549,10 +568,17 @@ class SharedPrefix:
             splits = max(1, min(48, -(-148 // layout.kv_heads), fit))
         if not 1 <= splits <= 63:
             raise ValueError("a shared prefix is cut into 1 to 63 splits")
-        sizes = (C.c_int64 * 2)()
-        _lib.call("oscar_shared_prefix_layout", max_reqs, max_tokens, hq, layout.kv_heads, C.addressof(sizes))
-        self.max_reqs, self.items, self.splits, self.hq = max_reqs, int(sizes[0]), splits, hq
-        self.plan = torch.empty(int(sizes[1]), dtype=torch.int32, device=device)
+        self.items, words = _shared_sizes(max_reqs, max_tokens, hq, layout.kv_heads)
+        self.max_reqs, self.max_tokens, self.splits, self.hq, self.layout = max_reqs, max_tokens, splits, hq, layout
+        self.plan = torch.empty(words, dtype=torch.int32, device=device)
+        self._geometry = None
+
+    def geometry(self, table_stride: int, query_tile: int):
+        geo = self._geometry
+        if geo is None or geo.table_stride != table_stride:
+            geo = self._geometry = geometry(self.layout, self.hq, table_stride)
+        geo.query_tile = query_tile
+        return geo
 
 
 def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
@@ -563,25 +589,80 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
     hold the same history, as after ``fork_requests``; -1: not in a group.  ``shared`` is a
     ``SharedPrefix`` to fill again (needed for graph capture of changing steps), else a new
     one.  Returns it, for ``decode_attention(..., shared=)``."""
-    for t, name in ((groups, "groups"), (prefix_lens, "prefix_lens")):
-        if t.dtype != torch.int32 or t.ndim != 1 or t.shape[0] < meta.num_reqs:
-            raise ValueError(f"{name} must be int32 with an entry per request")
+    if groups.dtype != torch.int32 or prefix_lens.dtype != torch.int32 or groups.ndim != 1 or prefix_lens.ndim != 1:
+        raise ValueError("groups and prefix_lens must be int32 with an entry per request")
     reqs = min(groups.shape[0], prefix_lens.shape[0], meta.max_num_reqs)
+    if reqs < meta.num_reqs:
+        raise ValueError("groups and prefix_lens must be int32 with an entry per request")
     if shared is None:
         tokens = getattr(meta, "num_actual_tokens", None) or meta.num_reqs * max(1, meta.max_query_len)
         shared = SharedPrefix(reqs, tokens, hq, layout, groups.device)
-    elif shared.hq != hq or shared.max_reqs < meta.num_reqs:
-        raise ValueError("the plan was made for other heads or fewer requests")
-    if reqs < shared.max_reqs:
+    elif shared.hq != hq or shared.max_reqs < meta.num_reqs or shared.layout != layout:
+        raise ValueError("the plan was made for other heads, another layout or fewer requests")
+    elif reqs < shared.max_reqs:
         raise ValueError(f"groups and prefix_lens must have the plan's {shared.max_reqs} entries")
-    device = _same_device(groups, prefix_lens, shared.plan, meta.counts)
-    groups, prefix_lens = groups.contiguous(), prefix_lens.contiguous()
+    table = meta.block_tables
+    device = _same_device(groups, prefix_lens, shared.plan, meta.counts, table)
+    groups, prefix_lens = _dense(groups), _dense(prefix_lens)
     with device:
         _lib.call("oscar_prepare_shared_prefix", meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
                   meta.counts.data_ptr(), groups.data_ptr(), prefix_lens.data_ptr(), shared.max_reqs, shared.items,
-                  shared.splits, geometry(layout, hq, meta.block_tables.stride(0)), shared.plan.data_ptr(),
-                  _stream(groups))
+                  shared.splits, shared.geometry(table.stride(0), layout.config.queries_per_tile),
+                  shared.plan.data_ptr(), _stream(groups))
     return shared
+
+
+def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale, splits, rv, output, scratch,
+                   store_window, shared):
+    """``decode_attention`` of a step with a plan."""
+    n, hq, _ = query.shape
+    if shared.hq != hq or shared.max_reqs < meta.num_reqs or shared.layout != layout:
+        raise ValueError("the plan was made for other heads, another layout or fewer requests")
+    if not scale > 0:
+        raise ValueError("a shared prefix needs a positive softmax scale")
+    if history.numel() % layout.stripe_page_bytes or not history.is_contiguous():
+        raise ValueError("the history view must be whole contiguous pages")
+    if output.dtype != torch.bfloat16 or not output.is_contiguous() or output.numel() != query.numel():
+        raise ValueError("output must be contiguous bf16 [n, Hq * 256]")
+    if qrot.shape != query.shape or qrot.dtype != torch.bfloat16 or rv.shape != (256, 256) or rv.dtype != torch.bfloat16:
+        raise ValueError("qrot must be bf16 like the query, and rv a bf16 [256, 256] rotation")
+    if key.shape != (n, layout.kv_heads, 256) or value.shape != key.shape:
+        raise ValueError("key and value must be [n, KV heads, 256]")
+    table = meta.block_tables
+    if table.stride(1) != 1:
+        raise ValueError("block table rows must be contiguous")
+    device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan, table)
+    if n == 0:
+        return output
+    splits = min(int(splits), 64 - shared.splits)
+    if splits < 1:
+        raise ValueError("a step needs at least one split")
+    slots = splits + shared.splits + 1
+    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != slots - 1:
+        rows = n * hq * slots
+        buffer = torch.empty(rows * 257, dtype=torch.float32, device=query.device)
+        partials = buffer.data_ptr()
+        lse = partials + rows * 1024
+    else:
+        partials, lse = scratch.partials.data_ptr(), scratch.lse.data_ptr()
+    query, key, value = _rows(query), _rows(key), _rows(value)
+    qrot, rv = _dense(qrot), _dense(rv)
+    tile = layout.config.queries_per_tile
+    max_q = getattr(meta, "max_query_len", None)
+    programs = min(attention_programs(n, meta.max_num_reqs, tile), meta.tasks.shape[0])
+    if isinstance(max_q, int) and 0 < max_q < tile:
+        tile = max_q
+    with device:
+        _lib.call("oscar_decode_attention_shared", qrot.data_ptr(), query.data_ptr(), query.stride(0), query.stride(1),
+                  key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+                  history.data_ptr(), history.numel() // layout.stripe_page_bytes, window.data_ptr(),
+                  meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), table.data_ptr(), meta.counts.data_ptr(),
+                  meta.tasks.data_ptr(), meta.task_count.data_ptr(), programs, n, rv.data_ptr(),
+                  shared.plan.data_ptr(), shared.max_reqs, shared.items, shared.splits, partials, lse,
+                  output.data_ptr(), shared.geometry(table.stride(0), tile), float(scale), splits,
+                  min(n, meta.max_num_reqs) if store_window else 0, _status(query), _stream(query))
+    _checked("oscar_decode_attention_shared", query)
+    return output
 
 
 def decode_attention(qrot, query, key, value, history, window, meta, layout, scale, splits, rv, output, scratch=None,
@@ -593,43 +674,20 @@ def decode_attention(qrot, query, key, value, history, window, meta, layout, sca
     attended once per group, and only the rest per request; ``splits`` is then at most
     64 - shared.splits (more is cut to that)."""
     if shared is not None:
-        if shared.hq != query.shape[1] or shared.max_reqs < meta.num_reqs:
-            raise ValueError("the plan was made for other heads or fewer requests")
-        if not scale > 0:
-            raise ValueError("a shared prefix needs a positive softmax scale")
-        if history.numel() % layout.stripe_page_bytes or not history.is_contiguous():
-            raise ValueError("the history view must be whole contiguous pages")
-        if output.dtype != torch.bfloat16 or not output.is_contiguous() or output.numel() != query.numel():
-            raise ValueError("output must be contiguous bf16 [n, Hq * 256]")
-        splits = min(int(splits), 64 - shared.splits)
-        device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan)
-    else:
-        _require_cuda(qrot, query, key, value, history, window, rv, output)
+        return _decode_shared(qrot, query, key, value, history, window, meta, layout, scale, splits, rv, output, scratch,
+                              store_window, shared)
+    _require_cuda(qrot, query, key, value, history, window, rv, output)
     n, hq, _ = query.shape
     if n == 0:
         return output
-    slots = splits + (shared.splits if shared is not None else 0)
-    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != slots:
-        scratch = DecodeScratch(n, hq, slots, query.device)
+    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != splits:
+        scratch = DecodeScratch(n, hq, splits, query.device)
     query, key, value = _rows(query), _rows(key), _rows(value)
     qrot = qrot.contiguous()
     rv = rv.contiguous()
     geo = _meta_common(meta, layout, hq)
     programs = min(attention_programs(n, meta.max_num_reqs, layout.config.queries_per_tile), meta.tasks.shape[0])
     window_programs = min(n, meta.max_num_reqs) if store_window else 0
-    if shared is not None:
-        with device:
-            _lib.call("oscar_decode_attention_shared", qrot.data_ptr(), query.data_ptr(), query.stride(0),
-                      query.stride(1), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-                      value.stride(1), history.data_ptr(), history.numel() // layout.stripe_page_bytes,
-                      window.data_ptr(), meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
-                      meta.block_tables.data_ptr(), meta.counts.data_ptr(), meta.tasks.data_ptr(),
-                      meta.task_count.data_ptr(), programs, n, rv.data_ptr(), shared.plan.data_ptr(), shared.max_reqs,
-                      shared.items, shared.splits, scratch.partials.data_ptr(), scratch.lse.data_ptr(),
-                      output.data_ptr(), geo, float(scale), int(splits), window_programs, _status(query),
-                      _stream(query))
-        _checked("oscar_decode_attention_shared", query)
-        return output
     _lib.call("oscar_decode_attention", qrot.data_ptr(), query.data_ptr(), query.stride(0), query.stride(1),
               key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
               history.data_ptr(), window.data_ptr(), meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
