@@ -100,15 +100,23 @@ OSCAR_DEVINL int block_scan(int v, int &total) {
   return v + (warp ? before : 0);
 }
 
-// list[0 .. found) = the lowest free pages, at most `want`; returns found.
+// list[0 .. found) = the lowest free pages, at most `want`; returns found.  Four pages per
+// thread and step (the counts are 16-byte aligned and padded).
 OSCAR_DEVINL int find_free(const Pool &p, int want) {
   int found = 0;
-  for (int base = 1; base < p.num_pages && found < want; base += kPlanThreads) {
-    const int page = base + threadIdx.x;
-    const bool is_free = page < p.num_pages && __ldcg(p.refs + page) == 0;
+  for (int base = 0; base < p.num_pages && found < want; base += 4 * kPlanThreads) {
+    const int page = base + 4 * threadIdx.x;
+    int4 c = make_int4(1, 1, 1, 1);
+    if (page < p.num_pages) c = __ldcg(reinterpret_cast<const int4 *>(p.refs + page));
+    const bool f[4] = {c.x == 0 && page > 0, c.y == 0 && page + 1 < p.num_pages, c.z == 0 && page + 2 < p.num_pages,
+                       c.w == 0 && page + 3 < p.num_pages};
+    const int mine = f[0] + f[1] + f[2] + f[3];
     int total;
-    const int at = found + block_scan(is_free, total) - 1;
-    if (is_free && at < want) p.list[at] = page;
+    int at = found + block_scan(mine, total) - mine;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (f[k] && at < want)
+        p.list[at++] = page + k;
     found += total;
   }
   __syncthreads();
@@ -256,67 +264,117 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyPara
 
 // ---- resize -----------------------------------------------------------------------
 
+// A warp takes 16 list entries at a time: lane k < 16 judges entry k, then the whole warp
+// walks the entries that change the table, the loads of four of them in flight.
+constexpr int kEntries = 16;
+
 __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Pool p, const int32_t *__restrict__ rows,
                                                               const int32_t *__restrict__ lens, int count,
                                                               int32_t *__restrict__ result) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kPlanThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = kEntries * kPlanThreads / 32;
   claim_rows(p, rows, count);
   // releases first: their pages serve the growth of the same call
-  for (int i = warp; i < count; i += warps) {
-    const int r = rows[i];
-    int state = -1;
-    if (r >= 0 && r < p.max_reqs && __ldcg(p.claim + r) == i) {
-      const int n = p.lens[r], want = lens[i];
-      if (want == 0 && n >= 0 && n <= row_tokens(p)) {
-        const int pages = pages_of(p, n), cols = pages * p.per_page;
-        int32_t *row = p.table + (int64_t)r * p.columns;
-        for (int c = lane; c < cols; c += 32) {
-          const int block = row[c];
-          if (c % p.per_page == 0 && page_ok(p, block / p.per_page)) atomicSub(p.refs + block / p.per_page, 1);
-          row[c] = 0;
+  for (int base = 0; base < count; base += step) {
+    const int i = base + warp * kEntries + lane;
+    int state = 0, cols = 0, r = 0;  // state 0: no entry, -1 refused, 1 release, 2 + pages needed
+    if (lane < kEntries && i < count) {
+      r = rows[i];
+      const int want = lens[i];
+      state = -1;
+      if (r >= 0 && r < p.max_reqs && __ldcg(p.claim + r) == i) {
+        const int n = p.lens[r];
+        if (want == 0 && n >= 0 && n <= row_tokens(p)) {
+          state = 1;
+          cols = pages_of(p, n) * p.per_page;
+          p.lens[r] = 0;
+        } else if (want > 0 && want >= n && n >= 0 && want <= row_tokens(p)) {
+          state = 2 + pages_of(p, want) - pages_of(p, n);
         }
-        state = 1;
-      } else if (want > 0 && want >= n && n >= 0 && want <= row_tokens(p)) {
-        state = 2 + pages_of(p, want) - pages_of(p, n);  // 2 + pages needed
       }
-    }
-    __syncwarp();
-    if (lane == 0) {
       result[i] = state;
-      if (state == 1) p.lens[r] = 0;
+    }
+    uint32_t left = __ballot_sync(0xffffffffu, cols > 0);
+    while (left) {
+      int32_t *row[4];
+      int n[4], most = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = left ? __ffs(left) - 1 : -1;
+        left &= left - 1;  // 0 stays 0
+        row[k] = p.table + (int64_t)__shfl_sync(0xffffffffu, r, e & 31) * p.columns;
+        n[k] = __shfl_sync(0xffffffffu, cols, e & 31);
+        if (e < 0) n[k] = 0;
+        most = max(most, n[k]);
+      }
+      for (int c = lane; c < most; c += 32) {
+        int block[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c < n[k]) block[k] = row[k][c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c < n[k]) {
+            if (c % p.per_page == 0 && page_ok(p, block[k] / p.per_page)) atomicSub(p.refs + block[k] / p.per_page, 1);
+            row[k][c] = 0;
+          }
+      }
     }
   }
   __syncthreads();
   int carry = 0;
   for (int base = 0; base < count; base += kPlanThreads) {
     const int i = base + threadIdx.x;
+    const int need = i < count ? result[i] - 2 : -1;  // < 0: nothing to grow
     int total;
-    const int upto = carry + block_scan(i < count ? max(result[i] - 2, 0) : 0, total);
-    if (i < count) {
-      p.jobs[i].src = upto;
-      p.jobs[i].tokens = result[i] - 2;  // pages needed; < 0: nothing to grow
-    }
+    const int upto = carry + block_scan(max(need, 0), total);
+    if (i < count) p.jobs[i].src = upto;
     carry += total;
   }
   __syncthreads();
   const int have = find_free(p, carry);
-  for (int i = warp; i < count; i += warps) {
-    const int need = p.jobs[i].tokens, upto = p.jobs[i].src;
-    if (need < 0) continue;  // released or refused
-    const bool ok = need == 0 || upto <= have;
-    if (ok) {
-      const int r = rows[i], from = pages_of(p, p.lens[r]);
-      int32_t *row = p.table + (int64_t)r * p.columns + (int64_t)from * p.per_page;
-      for (int c = lane; c < need * p.per_page; c += 32) {
-        const int page = p.list[upto - need + c / p.per_page];
-        row[c] = page * p.per_page + c % p.per_page;
-        if (c % p.per_page == 0) p.refs[page] = 1;
+  for (int base = 0; base < count; base += step) {
+    const int i = base + warp * kEntries + lane;
+    int first = 0, words = 0;  // first fresh page in the list, table words to write
+    int64_t at = 0;
+    if (lane < kEntries && i < count) {
+      const int need = result[i] - 2, upto = p.jobs[i].src;
+      if (need >= 0) {
+        const bool ok = need == 0 || upto <= have;
+        if (ok) {
+          const int r = rows[i];
+          first = upto - need, words = need * p.per_page;
+          at = (int64_t)r * p.columns + (int64_t)pages_of(p, p.lens[r]) * p.per_page;
+          p.lens[r] = lens[i];
+        }
+        result[i] = ok;
       }
     }
-    __syncwarp();
-    if (lane == 0) {
-      if (ok) p.lens[rows[i]] = lens[i];
-      result[i] = ok;
+    uint32_t left = __ballot_sync(0xffffffffu, words > 0);
+    while (left) {
+      int32_t *row[4];
+      int from[4], n[4], most = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = left ? __ffs(left) - 1 : -1;
+        left &= left - 1;
+        row[k] = p.table + __shfl_sync(0xffffffffu, at, e & 31);
+        from[k] = __shfl_sync(0xffffffffu, first, e & 31);
+        n[k] = __shfl_sync(0xffffffffu, words, e & 31);
+        if (e < 0) n[k] = 0;
+        most = max(most, n[k]);
+      }
+      for (int c = lane; c < most; c += 32) {
+        int page[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c < n[k]) page[k] = p.list[from[k] + c / p.per_page];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c < n[k]) {
+            row[k][c] = page[k] * p.per_page + c % p.per_page;
+            if (c % p.per_page == 0) p.refs[page[k]] = 1;
+          }
+      }
     }
   }
 }
