@@ -469,9 +469,9 @@ struct RawParams {
   float scale_log2;
   int32_t ntiles;
   // shared-prefix step: split slots [shared_base, shared_base + shared_slots) belong to the
-  // group's partials, of which request r has shared_used[r]; the others are marked empty here
+  // group's partials, of which request r < shared_reqs has shared_used[r]; the others are marked empty here
   const int32_t *shared_used;
-  int32_t shared_base, shared_slots;
+  int32_t shared_base, shared_slots, shared_reqs;
 };
 
 // Warps per CTA: 4 (three CTAs per SM), or 12 for the few CTAs of a small shared-prefix step,
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(32 * WARPS) raw_attention_kernel(RawParams P) 
     if (!live[r] || warp != 0) continue;
     if (gi == 0) P.lse[orow[r]] = L[r] > 0.f ? (M[r] * 0.69314718055994531f + logf(L[r])) : -INFINITY;
     if (P.shared_used)
-      for (int s = P.shared_used[ti.req] + gi; s < P.shared_slots; s += 8)
+      for (int s = (ti.req < P.shared_reqs ? P.shared_used[ti.req] : 0) + gi; s < P.shared_slots; s += 8)
         P.lse[orow[r] - P.split_index + P.shared_base + s] = -INFINITY;
   }
   // O^T fragment: m-tile mv rows (dims) 16mv + gi and 16mv + gi + 8
@@ -1402,6 +1402,7 @@ struct SharedStep {
   const int32_t *plan;
   int32_t max_reqs, items, splits;
   int64_t num_pages;
+  int32_t table_rows;
 };
 
 static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key, int64_t ks0,
@@ -1436,7 +1437,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     H.qstarts = qstarts, H.seq_lens = seq_lens, H.table = table, H.counts = counts;
     H.tasks = tasks, H.task_count = task_count, H.num_tasks = num_tasks;
     H.partials = scratch_partials, H.lse = scratch_lse, H.split_slots = all_splits + 1, H.splits = splits;
-    H.shared_end = shared_end;
+    H.shared_end = shared_end, H.shared_reqs = shared ? shared->max_reqs : 0;
     H.geo = geo;
     H.scale_log2 = scale * kLog2e;
     H.balanced = 1;
@@ -1459,7 +1460,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
       // requests have for themselves runs beside it
       SharedLaunch L{};
       L.query = reinterpret_cast<const __nv_bfloat16 *>(qrot);
-      L.history = history, L.num_pages = shared->num_pages;
+      L.history = history, L.num_pages = shared->num_pages, L.n = n, L.table_rows = shared->table_rows;
       L.table = table, L.plan = shared->plan, L.max_reqs = shared->max_reqs, L.items = shared->items;
       L.partials = scratch_partials, L.lse = scratch_lse, L.split_slots = all_splits + 1, L.slot_base = splits;
       L.geo = geo;
@@ -1482,7 +1483,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     R.tasks = tasks, R.task_count = task_count;
     R.partials = scratch_partials, R.lse = scratch_lse, R.split_slots = all_splits + 1, R.split_index = all_splits;
     if (shared) R.shared_used = shared_end + shared_up4(shared->max_reqs);
-    R.shared_base = splits, R.shared_slots = shared_splits;
+    R.shared_base = splits, R.shared_slots = shared_splits, R.shared_reqs = shared ? shared->max_reqs : 0;
     R.geo = geo;
     R.scale_log2 = scale * kLog2e;
     R.ntiles = (geo.query_tile * geo.group + 7) / 8;
@@ -1543,16 +1544,16 @@ extern "C" int oscar_decode_attention_shared(const void *qrot, const void *query
                                              const void *key, int64_t ks0, int64_t ks1, const void *value, int64_t vs0,
                                              int64_t vs1, const uint8_t *history, int64_t num_pages, void *window,
                                              const int32_t *qstarts, const int32_t *seq_lens, const int32_t *table,
-                                             const int32_t *counts, const int32_t *tasks, const int32_t *task_count,
-                                             int32_t num_tasks, int64_t n, const void *rv, const int32_t *plan,
+                                             int32_t table_rows, const int32_t *counts, const int32_t *tasks,
+                                             const int32_t *task_count, int32_t num_tasks, int64_t n, const void *rv, const int32_t *plan,
                                              int32_t plan_reqs, int32_t plan_items, int32_t plan_splits,
                                              float *scratch_partials, float *scratch_lse, void *output,
                                              oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
                                              int32_t *status, void *stream) {
-  if (!plan || plan_reqs < 1 || plan_items < 1 || plan_splits < 1 || plan_splits > 63 || num_pages < 1 ||
+  if (!plan || table_rows < 1 || plan_reqs < 1 || plan_items < 1 || plan_splits < 1 || plan_splits > 63 || num_pages < 1 ||
       num_pages > INT32_MAX || !(scale > 0.f))
     return OSCAR_ERR_INVALID;
-  const SharedStep shared{plan, plan_reqs, plan_items, plan_splits, num_pages};
+  const SharedStep shared{plan, plan_reqs, plan_items, plan_splits, num_pages, table_rows};
   return decode_step(qrot, query, qs0, qs1, key, ks0, ks1, value, vs0, vs1, history, window, qstarts, seq_lens, table,
                      counts, tasks, task_count, num_tasks, n, rv, scratch_partials, scratch_lse, output, geo, scale,
                      splits, window_programs, status, stream, &shared);

@@ -44,9 +44,10 @@ struct HistParams {
   // (-1: none); every bounded device wait gives up after wait_probes probes
   int32_t withhold;
   uint32_t wait_probes;
-  // end of the history that a request's group attends together (shared_prefix.cu), per
-  // request; null: nothing is shared
+  // end of the history that a request's group attends together (shared_prefix.cu), for the
+  // first shared_reqs requests; null: nothing is shared
   const int32_t *shared_end;
+  int32_t shared_reqs;
 };
 
 constexpr int kMinSplitTokens = 1024;
@@ -82,7 +83,7 @@ OSCAR_DEVINL TaskInfo load_task(int task, const int32_t *tasks, const int32_t *t
 // [sink_len, recent_begin) is the request's own part.
 OSCAR_DEVINL TaskInfo load_history_task(int task, const HistParams &P) {
   TaskInfo ti = load_task(task, P.tasks, P.task_count, P.qstarts, P.seq_lens, P.counts, P.geo);
-  if (ti.live && P.shared_end) ti.sink_len = max(ti.sink_len, min(P.shared_end[ti.req], ti.recent_begin));
+  if (ti.live && P.shared_end && ti.req < P.shared_reqs) ti.sink_len = max(ti.sink_len, min(P.shared_end[ti.req], ti.recent_begin));
   return ti;
 }
 

@@ -84,11 +84,12 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const PlanPar
   int32_t *s_tiles = sm + 3 * P.max_reqs;                     // group start: history tiles
   int32_t *s_seq = sm + 4 * P.max_reqs;                       // tokens of the request
   int32_t *s_tok = sm + 5 * P.max_reqs;                       // first token in the step
-  __shared__ int32_t s_cost[kPlanSpans], s_span[kPlanSpans], s_total, s_row_tiles, s_side, s_scan[kPlanWarps];
+  __shared__ int32_t s_cost[kPlanSpans], s_span[kPlanSpans], s_row_tiles, s_side, s_scan[kPlanWarps];
+  __shared__ unsigned long long s_total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t *ends = P.plan + kSharedHead, *used = ends + (P.max_reqs + 3) / 4 * 4;
   SharedItem *items = reinterpret_cast<SharedItem *>(used + (P.max_reqs + 3) / 4 * 4);
-  if (tid == 0) s_total = s_row_tiles = s_side = 0;
+  if (tid == 0) s_total = 0, s_row_tiles = s_side = 0;
   for (int r = tid; r < P.max_reqs; r += kPlanThreads) {
     int label = -1, limit = INT_MAX;
     if (r < nr) {
@@ -140,9 +141,10 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const PlanPar
   }
   __syncthreads();
   {
-    int mine = 0, mine_rows = 0, side = 0;
+    unsigned long long mine = 0;
+    int mine_rows = 0, side = 0;
     for (int r = tid; r < nr; r += kPlanThreads) {
-      mine += s_rows[r] * s_tiles[r], mine_rows += s_rows[r];
+      mine += (unsigned long long)s_rows[r] * s_tiles[r], mine_rows += s_rows[r];
       // what the request has for itself, once per task of query_tile queries
       const int qlen = s_tok[r + 1] - s_tok[r], own = max(0, s_seq[r] - max(0, ends[r] - g.sink));
       if (qlen > 0) {
@@ -151,25 +153,25 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const PlanPar
         side += (int)fminf(cost, 1e6f);
       }
     }
-    mine = warp_sum(mine), mine_rows = warp_sum(mine_rows), side = warp_sum(side);
-    if (lane == 0) atomicAdd(&s_side, side);
-    if (lane == 0 && mine_rows) atomicAdd(&s_total, mine), atomicAdd(&s_row_tiles, mine_rows);
+    if (mine) atomicAdd(&s_total, mine);  // few starts
+    mine_rows = warp_sum(mine_rows), side = warp_sum(side);
+    if (lane == 0) atomicAdd(&s_side, side), atomicAdd(&s_row_tiles, mine_rows);
   }
   __syncthreads();
-  const int64_t total = (int64_t)s_total * g.kv_heads;
-  if (total == 0 || s_row_tiles > P.items) {  // nothing shared, or more row tiles than the plan holds
+  if (s_total == 0 || s_row_tiles > P.items) {  // nothing shared, or more row tiles than the plan holds
     for (int r = tid; r < nr; r += kPlanThreads) ends[r] = 0, used[r] = 0;
     if (tid == 0) P.plan[0] = 0, P.plan[1] = P.sms;
     return;
   }
-  const int64_t side = (int64_t)s_side * g.kv_heads;
-  const int sms = P.sms - (int)min((int64_t)P.sms / 2, P.sms * side / (side + total));
-  // candidate spans: around one wave of CTAs, then 2 .. 17 waves; the
-  // cheapest in (waves x (longest split + fixed cost)) wins, the first among equals
+  // The choice of the split length only weighs costs: 32-bit arithmetic, saturated.
+  const uint32_t heads = g.kv_heads, total = (uint32_t)min(s_total * heads, 1ull << 30);
+  const float side = (float)s_side * heads;
+  const uint32_t sms = P.sms - (uint32_t)(min(0.5f, side / (side + total)) * P.sms);
+  // candidate spans: around one wave of CTAs, then 2 .. 17 waves; the cheapest in (waves x
+  // (longest split + fixed cost)) wins, the first among equals
   for (int c = warp; c < kPlanSpans; c += kPlanWarps) {
-    const int64_t base = max((int64_t)1, (total + sms - 1) / sms);
-    const int64_t want = c < 16 ? base + base * c / 16 : (base + c - 15) / (c - 14);
-    const int span = (int)min((int64_t)1 << 24, max((int64_t)1, want));
+    const uint32_t base = (total + sms - 1) / sms;
+    const int span = (int)(c < 16 ? base + base / 16 * c + base % 16 * c / 16 : (base + c - 15) / (c - 14));
     int count = 0, longest = 0;
     for (int r = lane; r < nr; r += 32) {
       if (!s_rows[r]) continue;
@@ -180,9 +182,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const PlanPar
     count = warp_sum(count);
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (lane == 0) {
-      const int64_t waves = ((int64_t)count * g.kv_heads + sms - 1) / sms;
-      const int64_t cost = waves * (longest + kItemCost);
-      s_cost[c] = count > P.items ? INT_MAX : (int)min((int64_t)INT_MAX - 1, cost);
+      const float waves = ceilf((float)count * heads / sms);
+      s_cost[c] = count > P.items ? INT_MAX : (int)fminf(waves * (longest + kItemCost), 2e9f);
       s_span[c] = span;
     }
   }
@@ -279,6 +280,9 @@ struct SpParams {
   oscar_geometry geo;
   float scale_log2;
   int32_t *status;
+  // a plan of another step must not reach outside this one's buffers
+  int64_t n;
+  int32_t table_rows;
   int32_t item_cap;
   int32_t withhold;
   uint32_t wait_probes;
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) shared_prefix_kernel(const __gr
     for (int64_t w = blockIdx.x; w < work && ok; w += ctas, ++n) {
       const SharedItem it = P.items[w / heads];
       const int head = (int)(w % heads);
-      const bool live = row < it.rows;
+      const bool live = row < it.rows && it.tok0 + (it.row0 + row) / g.group < P.n;
       const int64_t qrow = (int64_t)(it.tok0 + (it.row0 + row) / g.group) * heads * g.group + head * g.group +
                            (it.row0 + row) % g.group;
       const uint4 *q = reinterpret_cast<const uint4 *>(P.query + qrow * kDim) + 16 * half;
@@ -657,7 +661,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) shared_prefix_kernel(const __gr
       for (int64_t w = blockIdx.x; w < work; w += ctas) {
         const SharedItem it = P.items[w / heads];
         const int head = (int)(w % heads);
-        if (row < it.rows) {
+        if (row < it.rows && it.tok0 + (it.row0 + row) / g.group < P.n) {
           const int64_t qrow = (int64_t)(it.tok0 + (it.row0 + row) / g.group) * heads * g.group + head * g.group +
                                (it.row0 + row) % g.group;
           P.lse[qrow * P.split_slots + P.slot_base + it.slot] = -INFINITY;
@@ -674,11 +678,11 @@ __global__ void __launch_bounds__(kSpThreads, 1) shared_prefix_kernel(const __gr
         for (int64_t w = blockIdx.x; w < work && ok; w += ctas) {
           const SharedItem it = P.items[w / heads];
           const int head = (int)(w % heads);
-          const int32_t *row = P.table + (int64_t)it.leader * g.table_stride;
+          const int32_t *row = P.table + (int64_t)min((uint32_t)it.leader, (uint32_t)P.table_rows - 1) * g.table_stride;
           for (int t = it.tile0; t < it.tile1; ++t, ++T) {
             const int st = T % kSpStages;
             const int pos = t * kSharedTile;
-            const int64_t slot = (int64_t)row[pos / kKernelBlock] * kKernelBlock + pos % kKernelBlock;
+            const int64_t slot = (int64_t)row[min(pos / kKernelBlock, g.table_stride - 1)] * kKernelBlock + pos % kKernelBlock;
             if (T >= kSpStages && !sp_wait(&S.packed_empty[st], (T / kSpStages - 1) & 1, S, P)) {
               ok = false;
               break;
@@ -808,7 +812,7 @@ int shared_prefix_launch(const SharedLaunch &L, cudaStream_t stream, int priorit
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return OSCAR_ERR_INVALID;
   P.query = L.query;
-  P.table = L.table, P.plan = L.plan;
+  P.table = L.table, P.plan = L.plan, P.n = L.n, P.table_rows = L.table_rows;
   P.items = reinterpret_cast<const SharedItem *>(L.plan + kSharedHead + 2 * shared_up4(L.max_reqs));
   P.partials = L.partials, P.lse = L.lse, P.split_slots = L.split_slots, P.slot_base = L.slot_base;
   P.geo = g;

@@ -28,6 +28,8 @@ struct SharedLaunch {
   const __nv_bfloat16 *query;  // rotated, [n, hq, 256] contiguous
   const uint8_t *history;
   int64_t num_pages;
+  int64_t n;              // tokens of the step
+  int32_t table_rows;
   const int32_t *table, *plan;
   int32_t max_reqs, items;  // plan capacities
   float *partials, *lse;

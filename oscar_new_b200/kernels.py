@@ -287,9 +287,12 @@ def _output_rows(out, like):
     if out.stride(2) != 1 or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
         raise ValueError("output rows must be 16-byte aligned with unit inner stride")
     n, h, _ = out.shape
-    if (n > 1 and h > 1 and abs(out.stride(0)) < 256 and abs(out.stride(1)) < 256) or (
-            n > 1 and out.stride(0) == 0) or (h > 1 and out.stride(1) == 0):
-        raise ValueError("output rows overlap each other")
+    step = sorted((stride, size) for stride, size in ((out.stride(0), n), (out.stride(1), h)) if size > 1)
+    width = 256
+    for stride, size in step:
+        if stride < width:
+            raise ValueError("output rows overlap each other")
+        width = stride * (size - 1) + width
     return out
 
 
@@ -562,7 +565,7 @@ class SharedPrefix:
     scratch stays under ``scratch_bytes``."""
 
     def __init__(self, max_reqs: int, max_tokens: int, hq: int, layout, device, splits: int | None = None,
-                 scratch_bytes: int = 256 << 20):
+                 scratch_bytes: int = 256 << 20, _blank: bool = True):
         if splits is None:
             fit = scratch_bytes // max(max_tokens * hq * 256 * 4, 1)
             splits = max(1, min(48, -(-148 // layout.kv_heads), fit))
@@ -570,7 +573,8 @@ class SharedPrefix:
             raise ValueError("a shared prefix is cut into 1 to 63 splits")
         self.items, words = _shared_sizes(max_reqs, max_tokens, hq, layout.kv_heads)
         self.max_reqs, self.max_tokens, self.splits, self.hq, self.layout = max_reqs, max_tokens, splits, hq, layout
-        self.plan = torch.empty(words, dtype=torch.int32, device=device)
+        # a plan that was never filled shares nothing
+        self.plan = (torch.zeros if _blank else torch.empty)(words, dtype=torch.int32, device=device)
         self._geometry = None
 
     def geometry(self, table_stride: int, query_tile: int):
@@ -596,7 +600,7 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
         raise ValueError("groups and prefix_lens must be int32 with an entry per request")
     if shared is None:
         tokens = getattr(meta, "num_actual_tokens", None) or meta.num_reqs * max(1, meta.max_query_len)
-        shared = SharedPrefix(reqs, tokens, hq, layout, groups.device)
+        shared = SharedPrefix(reqs, tokens, hq, layout, groups.device, _blank=False)
     elif shared.hq != hq or shared.max_reqs < meta.num_reqs or shared.layout != layout:
         raise ValueError("the plan was made for other heads, another layout or fewer requests")
     elif reqs < shared.max_reqs:
@@ -638,7 +642,7 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
     if splits < 1:
         raise ValueError("a step needs at least one split")
     slots = splits + shared.splits + 1
-    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != slots - 1:
+    if scratch is None or scratch.partials.shape[0] < n or scratch.splits != slots - 1 or scratch.partials.shape[1] != hq:
         rows = n * hq * slots
         buffer = torch.empty(rows * 257, dtype=torch.float32, device=query.device)
         partials = buffer.data_ptr()
@@ -656,8 +660,8 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
         _lib.call("oscar_decode_attention_shared", qrot.data_ptr(), query.data_ptr(), query.stride(0), query.stride(1),
                   key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
                   history.data_ptr(), history.numel() // layout.stripe_page_bytes, window.data_ptr(),
-                  meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), table.data_ptr(), meta.counts.data_ptr(),
-                  meta.tasks.data_ptr(), meta.task_count.data_ptr(), programs, n, rv.data_ptr(),
+                  meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), table.data_ptr(), table.shape[0],
+                  meta.counts.data_ptr(), meta.tasks.data_ptr(), meta.task_count.data_ptr(), programs, n, rv.data_ptr(),
                   shared.plan.data_ptr(), shared.max_reqs, shared.items, shared.splits, partials, lse,
                   output.data_ptr(), shared.geometry(table.stride(0), tile), float(scale), splits,
                   min(n, meta.max_num_reqs) if store_window else 0, _status(query), _stream(query))

@@ -357,3 +357,26 @@ def test_refusals(cuda_lib):
     with pytest.raises(ValueError, match="whole contiguous pages"):
         kernels.decode_attention(b.qrot, b.q, b.k, b.v, b.history[:-160], b.window, b.meta, b.layout, 1 / 16, 8, b.rv,
                                  out, shared=plan)
+
+
+def test_plans_of_other_steps_reach_nothing_outside(cuda_lib):
+    """An unfilled plan shares nothing; a plan of a larger step, or of fewer requests than the
+    device counts say, stays inside this step's buffers."""
+    b = simple(6, 1300, lambda i: i, 1, 8, 1, seed=16)
+    want = b.run(shared=False).clone()
+    blank = kernels.SharedPrefix(6, 6, 8, b.layout, DEV)
+    got = b.run(shared=blank)
+    assert float((got.float() - want.float()).norm() / want.float().norm()) < 5e-3
+    small = simple(3, 500, lambda i: i, 1, 8, 1, seed=17)
+    stale = kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8)
+    scratch = kernels.DecodeScratch(4, 8, 8 + stale.splits, DEV)
+    guard = scratch.partials[3].fill_(3.0)
+    small.run(shared=stale, scratch=scratch)  # its rows mean nothing, the memory behind them does
+    torch.cuda.synchronize()
+    assert bool((guard == 3.0).all()) and kernels.read_status(DEV) == 0
+    # the first three requests are planned, the others go their own way
+    b.meta.num_reqs = 3
+    few = kernels.prepare_shared_prefix(b.meta, b.groups[:3], b.lens[:3], b.layout, 8)
+    b.meta.num_reqs = 3
+    b.check(b.run(shared=few))
+    assert few.max_reqs == 3

@@ -33,6 +33,8 @@ def args(n=3, hq=4, h=2, rotary=64):
     (dict(key_out=torch.zeros(3, 3, 256, dtype=torch.bfloat16)), "bf16 output"),
     (dict(key_out=torch.zeros(3, 2, 260, dtype=torch.bfloat16)[..., :256]), "16-byte aligned"),
     (dict(key_out=torch.zeros(1, 1, 256, dtype=torch.bfloat16).expand(3, 2, 256)), "overlap each other"),
+    (dict(key_out=torch.zeros(1024, dtype=torch.bfloat16).as_strided((3, 2, 256), (256, 256, 1))), "overlap each other"),
+    (dict(key_out=torch.zeros(1536, dtype=torch.bfloat16).as_strided((3, 2, 256), (512, 128, 1))), "overlap each other"),
 ])
 def test_bad_arguments_are_refused(change, text):
     with pytest.raises(ValueError, match=text):
