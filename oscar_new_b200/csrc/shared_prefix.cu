@@ -4,7 +4,7 @@
 // A group's rows (members x queries x query heads of a KV head) are packed into tiles of
 // 128 rows, and one CTA attends a tile to a run of 64-token history tiles of one KV head:
 //   packed slots   one 4-D TMA copy per tile (144 of a slot's 160 bytes, 64 tokens of one
-//                  head, no multicast) into a 4-stage ring;
+//                  head, no multicast) into a 6-stage ring;
 //   operands       four warps expand the keys and four the values into bf16 tiles
 //                  (128-byte swizzle): a token has only four levels bf16(c * s + z) per
 //                  vector, kept in two registers, and one PRMT whose selector nibbles come
@@ -29,11 +29,11 @@
 // and hold S back).  It issues from converged code with constant operands: an MMA whose
 // operands have to be moved into uniform registers first takes 70 to 94 cycles to issue
 // whatever its size, one with constant ones 32 (M 128, N 64, K 16), the tensor cores' rate.
-// // The range is the same for all rows
-// of a group: [sink, end), end = the shortest of the members' prefix lengths and recent
-// windows (oscar_prepare_shared_prefix); what lies behind it for a member stays with the
-// per-request kernels.  Tokens outside the range get zero levels (their slots may hold
-// anything) and -inf scores.  Split partials (normalised O, lse) join the merge of the step.
+// The range is the same for all rows of a group: [sink, end), end = the shortest of the
+// members' prefix lengths and recent windows (oscar_prepare_shared_prefix); what lies behind
+// it for a member stays with the per-request kernels.  Tokens outside the range get zero
+// levels (their slots may hold anything) and -inf scores.  Split partials (normalised O, lse)
+// join the merge of the step.
 //
 // Every wait is bounded; a wait that gives up sets the status word, the CTA's rows get
 // lse = -inf, copies in flight land and issued MMAs complete before tensor memory is freed.

@@ -348,6 +348,7 @@ def qk_norm_rope(query, key, q_weight, k_weight, positions, cos_sin, eps=1e-6, w
         raise ValueError("counts are int32 [requests, active tokens]")
     if not float(eps) >= 0.0:
         raise ValueError("eps must not be negative")
+    counts = None if counts is None else _dense(counts)
     qo, ko = _output_rows(query_out, query), _output_rows(key_out, key)
     if query_out is not None or key_out is not None:
         same = [o.data_ptr() == i.data_ptr() and o.stride() == i.stride() for o, i in ((qo, query), (ko, key))]
@@ -591,8 +592,9 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
     groups, prefix_lens: int32 device tensors [requests].  Consecutive requests with the
     same label >= 0 form a group whose first ``prefix_lens`` tokens (the shortest counts)
     hold the same history, as after ``fork_requests``; -1: not in a group.  ``shared`` is a
-    ``SharedPrefix`` to fill again (needed for graph capture of changing steps), else a new
-    one.  Returns it, for ``decode_attention(..., shared=)``."""
+    ``SharedPrefix`` to fill again (needed for graph capture of changing steps; in stream
+    order, behind the steps that read it), else a new one.  Returns it, for
+    ``decode_attention(..., shared=)``."""
     if groups.dtype != torch.int32 or prefix_lens.dtype != torch.int32 or groups.ndim != 1 or prefix_lens.ndim != 1:
         raise ValueError("groups and prefix_lens must be int32 with an entry per request")
     reqs = min(groups.shape[0], prefix_lens.shape[0], meta.max_num_reqs)
@@ -635,7 +637,8 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
     table = meta.block_tables
     if table.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
-    device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan, table)
+    device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan, table,
+                          None if scratch is None else scratch.partials)
     if n == 0:
         return output
     splits = min(int(splits), 64 - shared.splits)

@@ -161,3 +161,14 @@ def test_captured_replays_follow_their_inputs(cuda_lib):
         graph.replay()
         check(qo, formula(q, w, 0.0, 1e-6, tab[pos], 128, False))
         check(ko, formula(k, w, 0.0, 1e-6, tab[pos], 128, False))
+
+
+def test_strided_counts(cuda_lib):
+    q = torch.randn(6, 4, 256, generator=torch.Generator().manual_seed(5)).bfloat16().to(DEV)
+    k = q[:, :2].contiguous()
+    w, tab = torch.ones(256, device=DEV), table(10, 64)
+    pos = torch.arange(6, device=DEV)
+    qo, ko = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+    counts = torch.tensor([2, 6, 3, 6], dtype=torch.int32, device=DEV)[::2]  # 3 active tokens
+    kernels.qk_norm_rope(q, k, w, w, pos, tab, counts=counts, query_out=qo, key_out=ko)
+    assert bool((qo[3:] == 7).all()) and not bool((qo[2] == 7).any())

@@ -141,3 +141,21 @@ def test_captured_steps_replay_on_new_lists(cuda_lib):
         assert summary.tolist() == [live, len(copies)] and to.tolist() == where
         p.state()
         p.bytes()
+
+
+def test_caches_of_several_layers_repeat_a_call_from_one_state(cuda_lib):
+    layout = CacheLayout(768, 2, config=make_config(4, 64))
+    p = Pair(30, 6, 5000, layout, seed=9)
+    p.resize([0, 3], [4100, 900])
+    layers = [(p.history.clone(), p.window.clone()) for _ in range(2)]
+    for call in (lambda h, w: kernels.fork_requests(p.pool, p.ints([0, 3, 0]), p.ints([1, 2, 5]), h, w),
+                 lambda h, w: kernels.compact_pages(p.pool, h, w)[0]):
+        before, seen = p.pool.state.clone(), []
+        for h, w in layers:
+            p.pool.state.copy_(before)
+            seen.append((call(h, w), p.pool.state.clone()))
+        assert all(torch.equal(x, y) for x, y in zip(*seen)) and not torch.equal(seen[0][1], before)
+        assert torch.equal(layers[0][0], layers[1][0])
+        assert torch.equal(layers[0][1].view(torch.int16), layers[1][1].view(torch.int16))
+        kernels.resize_requests(p.pool, p.ints([0]), p.ints([0]))  # holes for the second call
+    assert not torch.equal(layers[0][0], p.history)

@@ -380,3 +380,10 @@ def test_plans_of_other_steps_reach_nothing_outside(cuda_lib):
     b.meta.num_reqs = 3
     b.check(b.run(shared=few))
     assert few.max_reqs == 3
+
+
+def test_scratch_of_another_device_is_refused(cuda_lib):
+    b = simple(4, 500, lambda i: i, 1, 8, 1, seed=19)
+    plan = kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8)
+    with pytest.raises((ValueError, RuntimeError), match="devices|CUDA device only"):
+        b.run(shared=plan, scratch=kernels.DecodeScratch(4, 8, 8 + plan.splits, "cpu"))
