@@ -11,7 +11,9 @@
 // in one block, and only the pages' bytes and table rows are spread over the GPU.
 //
 // Bytes: a page's used slots (tokens * H * 160, contiguous in the K stripe) and, for a
-// first page, the window (contiguous in the V stripe) are moved as 16 KiB slices.
+// first page, the window (contiguous in the V stripe) are moved as 16 KiB slices: 131 MB (read
+// and written) of 60 forks in 28 us, 4.7 TB/s, behind 8 us of decisions.  The next slice's job
+// fetched ahead of this one's stores, without the division: 28 us, not kept.
 #include <algorithm>
 
 #include "common.cuh"
@@ -265,7 +267,10 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyPara
 // ---- resize -----------------------------------------------------------------------
 
 // A warp takes 16 list entries at a time: lane k < 16 judges entry k, then the whole warp
-// walks the entries that change the table, the loads of four of them in flight.
+// walks the entries that change the table, the loads of four of them in flight and a lane per
+// page of a released row.  512 entries, 192 releases of 11 pages and 320 growths by 3 (one
+// block): 19 us; a lane per table word of a released row, each divided by the blocks of a
+// page, 24 us.
 constexpr int kEntries = 16;
 
 __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Pool p, const int32_t *__restrict__ rows,
@@ -306,18 +311,20 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Pool p, cons
         if (e < 0) n[k] = 0;
         most = max(most, n[k]);
       }
-      for (int c = lane; c < most; c += 32) {
+      for (int c = lane * p.per_page; c < most; c += 32 * p.per_page) {  // a lane per page
         int block[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (c < n[k]) block[k] = row[k][c];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (c < n[k]) {
-            if (c % p.per_page == 0 && page_ok(p, block[k] / p.per_page)) atomicSub(p.refs + block[k] / p.per_page, 1);
-            row[k][c] = 0;
-          }
+          if (c < n[k] && page_ok(p, block[k] / p.per_page)) atomicSub(p.refs + block[k] / p.per_page, 1);
       }
+      __syncwarp();  // the blocks are read
+      for (int c = lane; c < most; c += 32)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c < n[k]) row[k][c] = 0;
     }
   }
   __syncthreads();
