@@ -11,9 +11,9 @@
 // in one block, and only the pages' bytes and table rows are spread over the GPU.
 //
 // Bytes: a page's used slots (tokens * H * 160, contiguous in the K stripe) and, for a
-// first page, the window (contiguous in the V stripe) are moved as 16 KiB slices: 131 MB (read
-// and written) of 60 forks in 28 us, 4.7 TB/s, behind 8 us of decisions.  The next slice's job
-// fetched ahead of this one's stores, without the division: 28 us, not kept.
+// first page, the window (contiguous in the V stripe) are moved as 16 KiB slices: 131 MB (most of
+// it written) of 60 forks in 28 us, 4.6 TB/s, behind 8 us of decisions; 145 MB of a compaction
+// in 24 us.  The next slice's job fetched ahead of this one's stores: 28 us too, not kept.
 #include <algorithm>
 
 #include "common.cuh"
