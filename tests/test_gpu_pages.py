@@ -84,11 +84,11 @@ def test_random_steps(cuda_lib, block, heads, sink, recent, mtp):
 @pytest.mark.parametrize("tokens", [1, 127, 767, 768, 769, 1536, 1537, 3000])
 def test_fork_lengths_around_the_page_edges(cuda_lib, tokens):
     layout = CacheLayout(768, kv_heads=2, config=make_config(4, 64))
-    p = Pair(40, 8, 3072, layout, seed=tokens)
+    p = Pair(40, 8, 3500, layout, seed=tokens)
     p.resize([5, 2], [tokens, 900])
     p.fork([5, 5, 2, 5], [0, 1, 3, 7])
     p.fork([0, 7], [4, 6])  # forks of forks
-    p.resize([5, 0], [0, min(tokens + 800, 3072)])  # the first parent ends, its children live on
+    p.resize([5, 0], [0, min(tokens + 800, 3500)])  # the first parent ends, its children live on
     p.compact()
 
 
