@@ -387,3 +387,17 @@ def test_scratch_of_another_device_is_refused(cuda_lib):
     plan = kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8)
     with pytest.raises((ValueError, RuntimeError), match="devices|CUDA device only"):
         b.run(shared=plan, scratch=kernels.DecodeScratch(4, 8, 8 + plan.splits, "cpu"))
+
+
+@pytest.mark.parametrize("active", [1, 3, 7])
+def test_padded_step(cuda_lib, active):
+    """Requests behind the device counts take no part: their rows get what the step without
+    sharing gives them, and the others' rows are those of a step of their own."""
+    b = simple(8, 900, lambda i: 20 * i, 1, 8, 1, seed=20)
+    b.meta.counts.copy_(torch.tensor([active, active], dtype=torch.int32))
+    b.meta.task_count.fill_(active)
+    got, plain = b.run().clone(), b.run(shared=False)
+    want = b.exact()[0][:active]
+    # the bound that check() puts on a whole step
+    assert float((got[:active].double() - want).norm() / want.norm()) < 3.5e-3
+    assert torch.equal(got[active:], plain[active:]) and kernels.read_status(DEV) == 0
