@@ -305,20 +305,20 @@ int oscar_prepare_shared_prefix(const int32_t *qstarts, const int32_t *seq_lens,
                                 int32_t splits, oscar_geometry geo, int32_t *plan, void *stream);
 
 /* oscar_decode_attention for a step with a plan: num_pages pages of the cache, table_rows
- * rows of the block table, the plan
- * with the capacities and split count it was filled with (splits + plan_splits <= 64),
- * scale > 0.  Scratch rows hold splits + plan_splits + 1 partials.  The merged history row
- * is kept to about 16 bits through the inverse rotation and the output rounded once. */
+ * rows of the block table, the plan with the capacities and split count it was filled with
+ * (splits + plan_splits <= 64), scale > 0.  rv lies by rows, or by columns (rv_columns).
+ * Scratch rows hold splits + plan_splits + 1 partials.  The merged history row is kept to
+ * about 16 bits through the inverse rotation and the output rounded once. */
 int oscar_decode_attention_shared(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key,
                                   int64_t ks0, int64_t ks1, const void *value, int64_t vs0, int64_t vs1,
                                   const uint8_t *history, int64_t num_pages, void *window, const int32_t *qstarts,
                                   const int32_t *seq_lens, const int32_t *table, int32_t table_rows,
                                   const int32_t *counts, const int32_t *tasks, const int32_t *task_count,
-                                  int32_t num_tasks, int64_t n, const void *rv, const int32_t *plan,
-                                  int32_t plan_reqs, int32_t plan_items, int32_t plan_splits,
-                                  float *scratch_partials, float *scratch_lse, void *output, oscar_geometry geo,
-                                  float scale, int32_t splits, int32_t window_programs, int32_t *status,
-                                  void *stream);
+                                  int32_t num_tasks, int64_t n, const void *rv, int32_t rv_columns,
+                                  const int32_t *plan, int32_t plan_reqs, int32_t plan_items,
+                                  int32_t plan_splits, float *scratch_partials, float *scratch_lse, void *output,
+                                  oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
+                                  int32_t *status, void *stream);
 
 /* ---- page pool (no reference counterpart: there the host engine owns the pages and
  * shared pages are refused, backend.py:41-64) ----------------------------------------

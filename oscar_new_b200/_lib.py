@@ -84,7 +84,7 @@ _SIGNATURES = {
     "oscar_shared_prefix_layout": [I32, I64, I32, I32, P],
     "oscar_prepare_shared_prefix": [P, P, P, P, P, I32, I32, I32, Geometry, P, P],
     "oscar_decode_attention_shared": [P, P, I64, I64, P, I64, I64, P, I64, I64, P, I64, P, P, P, P, I32, P, P, P, I32, I64, P,
-                                      P, I32, I32, I32, P, P, P, Geometry, F32, I32, I32, P, P],
+                                      I32, P, I32, I32, I32, P, P, P, Geometry, F32, I32, I32, P, P],
     "oscar_page_pool_layout": [I32, I32, I32, P],
     "oscar_fork_requests": [P, I32, I32, I32, P, P, I32, P, P, Geometry, P, P],
     "oscar_resize_requests": [P, I32, I32, I32, I32, P, P, I32, P, P],

@@ -476,7 +476,7 @@ struct RawParams {
 
 // Warps per CTA: 4 (three CTAs per SM), or 12 for the few CTAs of a small shared-prefix step,
 // whose tokens then pass in a third of the steps (4 requests x 321 tokens, one KV head: the
-// step takes 43.7 us, 44.7 with 4).
+// step takes 41 us, one more with 4).
 constexpr int kRawWarps = 4, kRawWideWarps = 12;
 constexpr int raw_smem(int warps) { return warps * 2 * 16 * kDim * 2; }  // per warp K and V 16-token tiles
 
@@ -771,6 +771,7 @@ struct FinalParams {
   int32_t hq;
   const int32_t *counts;
   const __nv_bfloat16 *rv;
+  int32_t rv_columns;  // Rv lies by columns (finalize_wide_kernel only)
   __nv_bfloat16 *out;
 };
 
@@ -982,13 +983,15 @@ __global__ void __launch_bounds__(kFinWideThreads, 1) finalize_wide_kernel(Final
   __nv_bfloat16 *sA = sB + kDim * kDim;                             // hi rows, then lo rows
   float *s_la = reinterpret_cast<float *>(sA + 2 * kFinWideRows * kDim), *s_lb = s_la + kFinWideRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Rv rows in two halves of k: the first product waits for half of them
+  // Rv in two halves of k, the first product waits for one: [n][k] as rows, or [k][n] when it
+  // lies by columns (ldmatrix then transposes)
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
     for (int i = 0; i < kDim * 16 / kFinWideThreads; ++i) {
-      const int c = threadIdx.x + i * kFinWideThreads, n = c >> 4, ch = 16 * h + (c & 15);
-      cp_async_16(smem_u32(sB + n * kDim + ((ch ^ (n & 7)) << 3)), P.rv + n * kDim + ch * 8);
+      const int c = threadIdx.x + i * kFinWideThreads;
+      const int line = P.rv_columns ? 128 * h + (c >> 5) : c >> 4, ch = P.rv_columns ? c & 31 : 16 * h + (c & 15);
+      cp_async_16(smem_u32(sB + line * kDim + ((ch ^ (line & 7)) << 3)), P.rv + line * kDim + ch * 8);
     }
     cp_async_commit();
   }
@@ -1062,8 +1065,11 @@ __global__ void __launch_bounds__(kFinWideThreads, 1) finalize_wide_kernel(Final
       const int ar = lane & 15, ak = 16 * kk + (lane >> 4) * 8;
       ldmatrix_x4(ah, smem_u32(sA + a_index(ar, ak)));
       ldmatrix_x4(al, smem_u32(sA + kFinWideRows * kDim + a_index(ar, ak)));
-      const int n = 16 * warp + (lane >> 4) * 8 + (lane & 7), k = 16 * kk + ((lane >> 3) & 1) * 8;
-      ldmatrix_x4(b, smem_u32(sB + n * kDim + (((k >> 3) ^ (n & 7)) << 3)));
+      const int n = 16 * warp + (lane >> 4) * 8, k = 16 * kk + ((lane >> 3) & 1) * 8, in = lane & 7;
+      if (P.rv_columns)
+        ldmatrix_x4_trans(b, smem_u32(sB + (k + in) * kDim + (((n >> 3) ^ in) << 3)));
+      else
+        ldmatrix_x4(b, smem_u32(sB + (n + in) * kDim + (((k >> 3) ^ in) << 3)));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mma_bf16_16816(c[j], ah[0], ah[1], ah[2], ah[3], b[2 * j], b[2 * j + 1]);
@@ -1403,7 +1409,7 @@ struct SharedStep {
   const int32_t *plan;
   int32_t max_reqs, items, splits;
   int64_t num_pages;
-  int32_t table_rows;
+  int32_t table_rows, rv_columns;
 };
 
 static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t qs1, const void *key, int64_t ks0,
@@ -1511,6 +1517,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     if (!ensure_dynamic_smem<finalize_wide_kernel>(kFinWideSmem)) return OSCAR_ERR_LAUNCH;
     const WindowParams W{reinterpret_cast<const __nv_bfloat16 *>(key), reinterpret_cast<const __nv_bfloat16 *>(value),
                          ks0, ks1, vs0, vs1, reinterpret_cast<__nv_bfloat16 *>(window), qstarts, seq_lens, table, geo};
+    F.rv_columns = shared->rv_columns;
     const int row_blocks = (int)((F.rows + kFinWideRows - 1) / kFinWideRows);
     finalize_wide_kernel<<<row_blocks + window_programs, kFinWideThreads, kFinWideSmem, st>>>(F, W, row_blocks);
     window_done = true;
@@ -1546,15 +1553,15 @@ extern "C" int oscar_decode_attention_shared(const void *qrot, const void *query
                                              int64_t vs1, const uint8_t *history, int64_t num_pages, void *window,
                                              const int32_t *qstarts, const int32_t *seq_lens, const int32_t *table,
                                              int32_t table_rows, const int32_t *counts, const int32_t *tasks,
-                                             const int32_t *task_count, int32_t num_tasks, int64_t n, const void *rv, const int32_t *plan,
-                                             int32_t plan_reqs, int32_t plan_items, int32_t plan_splits,
-                                             float *scratch_partials, float *scratch_lse, void *output,
+                                             const int32_t *task_count, int32_t num_tasks, int64_t n, const void *rv,
+                                             int32_t rv_columns, const int32_t *plan, int32_t plan_reqs, int32_t plan_items,
+                                             int32_t plan_splits, float *scratch_partials, float *scratch_lse, void *output,
                                              oscar_geometry geo, float scale, int32_t splits, int32_t window_programs,
                                              int32_t *status, void *stream) {
   if (!plan || table_rows < 1 || plan_reqs < 1 || plan_items < 1 || plan_splits < 1 || plan_splits > 63 || num_pages < 1 ||
       num_pages > INT32_MAX || !(scale > 0.f))
     return OSCAR_ERR_INVALID;
-  const SharedStep shared{plan, plan_reqs, plan_items, plan_splits, num_pages, table_rows};
+  const SharedStep shared{plan, plan_reqs, plan_items, plan_splits, num_pages, table_rows, rv_columns};
   return decode_step(qrot, query, qs0, qs1, key, ks0, ks1, value, vs0, vs1, history, window, qstarts, seq_lens, table,
                      counts, tasks, task_count, num_tasks, n, rv, scratch_partials, scratch_lse, output, geo, scale,
                      splits, window_programs, status, stream, &shared);

@@ -653,7 +653,9 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
     else:
         partials, lse = scratch.partials.data_ptr(), scratch.lse.data_ptr()
     query, key, value = _rows(query), _rows(key), _rows(value)
-    qrot, rv = _dense(qrot), _dense(rv)
+    qrot = _dense(qrot)
+    columns = rv.stride() == (1, 256)  # a transposed rotation, as it lies
+    rv = rv if columns else _dense(rv)
     tile = layout.config.queries_per_tile
     max_q = getattr(meta, "max_query_len", None)
     programs = min(attention_programs(n, meta.max_num_reqs, tile), meta.tasks.shape[0])
@@ -665,7 +667,7 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
                   history.data_ptr(), history.numel() // layout.stripe_page_bytes, window.data_ptr(),
                   meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(), table.data_ptr(), table.shape[0],
                   meta.counts.data_ptr(), meta.tasks.data_ptr(), meta.task_count.data_ptr(), programs, n, rv.data_ptr(),
-                  shared.plan.data_ptr(), shared.max_reqs, shared.items, shared.splits, partials, lse,
+                  int(columns), shared.plan.data_ptr(), shared.max_reqs, shared.items, shared.splits, partials, lse,
                   output.data_ptr(), shared.geometry(table.stride(0), tile), float(scale), splits,
                   min(n, meta.max_num_reqs) if store_window else 0, _status(query), _stream(query))
     _checked("oscar_decode_attention_shared", query)

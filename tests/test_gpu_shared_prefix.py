@@ -401,3 +401,14 @@ def test_padded_step(cuda_lib, active):
     # the bound that check() puts on a whole step
     assert float((got[:active].double() - want).norm() / want.norm()) < 3.5e-3
     assert torch.equal(got[active:], plain[active:]) and kernels.read_status(DEV) == 0
+
+
+def test_rotation_by_rows_columns_and_strides(cuda_lib):
+    b = simple(5, 700, lambda i: i, 4, 24, 4, seed=21)
+    want = b.run().clone()
+    b.rv = b.rv.t().contiguous().t()
+    assert b.rv.stride() == (1, 256) and torch.equal(b.run(), want)
+    wide = torch.zeros(256, 512, dtype=torch.bfloat16, device=DEV)
+    wide[:, ::2] = b.rv
+    b.rv = wide[:, ::2]
+    assert torch.equal(b.run(), want)

@@ -105,7 +105,7 @@ def test_c_entries_refuse_before_any_launch():
                 dict(n=0), dict(n=64), dict(plan=None), dict(plan=p + 4)):
         assert prep(**bad) == 1, bad
     names = dict(qrot=p, q=p, qs0=6144, qs1=256, k=p, ks0=1024, ks1=256, v=p, vs0=1024, vs1=256, hist=p, pages=4, win=p,
-                 qst=p, seq=p, tab=p, rows=3, counts=p, tasks=p, tc=p, nt=3, n=3, rv=p, plan=p, reqs=3, items=10, ps=8,
+                 qst=p, seq=p, tab=p, rows=3, counts=p, tasks=p, tc=p, nt=3, n=3, rv=p, rvc=0, plan=p, reqs=3, items=10, ps=8,
                  part=p, lse=p, out=p, geo=geo, scale=0.1, splits=8, wp=3, status=None, stream=None)
     call = lambda **k: lib.oscar_decode_attention_shared(*{**names, **k}.values())  # noqa: E731
     for bad in (dict(plan=None), dict(reqs=0), dict(items=0), dict(ps=0), dict(ps=64), dict(pages=0), dict(pages=1 << 31),
