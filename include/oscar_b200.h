@@ -43,7 +43,8 @@ enum {
  * flight land, frees its tensor memory and returns, leaving the context usable.  The
  * library never clears the word: the caller zeroes it, and reads it after synchronising
  * the stream (a nonzero value means the outputs of the calls since it was zeroed are not
- * valid).  Launch-time errors are still the return value. */
+ * valid).  Launch-time errors are still the return value.  OSCAR_ERR_INVALID in the word is
+ * data that only the device sees and that the call does not hold for. */
 
 /* Cache geometry shared by the paged kernels (reference oscar_ascend/layout.py:8-95,
  * config.py:46-63).  page_bytes = physical_block_tokens * kv_heads * head_dim * 2. */
@@ -59,9 +60,15 @@ typedef struct oscar_geometry {
   int32_t recent;             /* R                                  */
   int32_t ring;               /* C = R + MTP + 1                    */
   int32_t table_stride;       /* row stride of the block table      */
-  int32_t query_tile;         /* QT: queries per task               */
+  int32_t query_tile;         /* QT: queries per task (see below)   */
   int64_t page_bytes;         /* J                                  */
 } oscar_geometry;
+
+/* query_tile of an attention launch may be less than the task table's when no request of
+ * the step has more queries (fewer rows to cover).  That is a promise about the device
+ * data, also of a captured launch's replays: queries of a task behind query_tile are not
+ * attended, their raw lse and so their output rows are NaN, and OSCAR_ERR_INVALID goes to
+ * the status word. */
 
 /* Percentile / factor clip parameters of one quantised stream (K or V).
  * mode 0 = percentile, 1 = factor; enabled 0 disables clipping.  For percentile mode

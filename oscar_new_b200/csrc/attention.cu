@@ -472,6 +472,7 @@ struct RawParams {
   // group's partials, of which request r < shared_reqs has shared_used[r]; the others are marked empty here
   const int32_t *shared_used;
   int32_t shared_base, shared_slots, shared_reqs;
+  int32_t *status;  // nullable error word
 };
 
 // Warps per CTA: 4 (three CTAs per SM), or 12 for the few CTAs of a small shared-prefix step,
@@ -494,6 +495,23 @@ OSCAR_DEVINL const __nv_bfloat16 *raw_token_row(const RawParams &P, const TaskIn
                  : P.value + (int64_t)cur * P.vs0 + (int64_t)head * P.vs1;
 }
 
+// A task's queries behind the launch's query_tile, up to the next task of its request: the
+// launch was made for shorter runs (a step captured for one query per request, say, and
+// replayed on longer ones), so none of its kernels attends them.  Their raw lse becomes NaN,
+// which every merge carries into the output rows, and the status word says so.
+OSCAR_DEVINL void refuse_uncovered(const RawParams &P, const TaskInfo &ti, int task, int head) {
+  const oscar_geometry &g = P.geo;
+  const int first = ti.qoff + g.query_tile;
+  int end = ti.qlen;
+  if (task + 1 < P.task_count[0] && P.tasks[2 * (task + 1)] == ti.req) end = min(end, P.tasks[2 * (task + 1) + 1]);
+  if (first >= end) return;
+  for (int i = threadIdx.x; i < (end - first) * g.group; i += blockDim.x) {
+    const int64_t row = (int64_t)(ti.qstart + first + i / g.group) * g.kv_heads * g.group + head * g.group + i % g.group;
+    P.lse[row * P.split_slots + P.split_index] = __int_as_float(0x7fffffff);
+  }
+  if (threadIdx.x == 0 && P.status) atomicMax(P.status, OSCAR_ERR_INVALID);
+}
+
 template <int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) raw_attention_kernel(RawParams P) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -505,6 +523,7 @@ __global__ void __launch_bounds__(32 * WARPS) raw_attention_kernel(RawParams P) 
   if (!ti.live || ti.qlen <= 0) return;
   const int rows_valid = min(g.query_tile, ti.qlen - ti.qoff) * g.group;
   if (8 * ntile >= rows_valid) return;
+  if (ntile == 0 && ti.qlen - ti.qoff > g.query_tile) refuse_uncovered(P, ti, task, head);
   const int nprev = ti.sink_len + ti.prefix - ti.recent_begin;
   const int total = nprev + ti.qlen;
   const int64_t owner = (int64_t)P.table[(int64_t)ti.req * g.table_stride] / (g.block_tokens / kKernelBlock);
@@ -1344,6 +1363,7 @@ extern "C" int oscar_attention_partials(const void *query, int64_t qs0, int64_t 
     P.geo = geo;
     P.scale_log2 = scale * kLog2e;
     P.ntiles = (geo.query_tile * geo.group + 7) / 8;
+    P.status = status;
     return raw_launch(P, num_tasks, (cudaStream_t)stream);
   }
   if (!history) return OSCAR_ERR_INVALID;
@@ -1494,6 +1514,7 @@ static int decode_step(const void *qrot, const void *query, int64_t qs0, int64_t
     R.geo = geo;
     R.scale_log2 = scale * kLog2e;
     R.ntiles = (geo.query_tile * geo.group + 7) / 8;
+    R.status = status;
     rc = raw_launch(R, num_tasks, side ? side->stream : st);
     if (rc) return rc;
     if (side && window_programs > 0 && !shared) {

@@ -453,6 +453,7 @@ def _meta_common(meta, layout, hq):
         raise ValueError("block table rows must be contiguous")
     # Launch only the query-row tiles this step can use: a task never holds more than
     # min(queries_per_tile, max_query_len) queries (host scheduler value, no device read).
+    # The raw kernel checks that on the device: queries past it become NaN, status word 1.
     max_q = getattr(meta, "max_query_len", None)
     if isinstance(max_q, int) and max_q > 0:
         geo.query_tile = min(geo.query_tile, max_q)
@@ -593,7 +594,9 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
     same label >= 0 form a group whose first ``prefix_lens`` tokens (the shortest counts)
     hold the same history, as after ``fork_requests``; -1: not in a group.  ``shared`` is a
     ``SharedPrefix`` to fill again (needed for graph capture of changing steps; in stream
-    order, behind the steps that read it), else a new one.  Returns it, for
+    order, behind the steps that read it), else a new one.  Labels, lengths and query
+    lengths may change from replay to replay, the last up to the ``meta.max_query_len`` that
+    ``decode_attention`` was captured with.  Returns it, for
     ``decode_attention(..., shared=)``."""
     if groups.dtype != torch.int32 or prefix_lens.dtype != torch.int32 or groups.ndim != 1 or prefix_lens.ndim != 1:
         raise ValueError("groups and prefix_lens must be int32 with an entry per request")
@@ -681,7 +684,11 @@ def decode_attention(qrot, query, key, value, history, window, meta, layout, sca
 
     ``shared`` (``prepare_shared_prefix``): the history that groups of requests share is
     attended once per group, and only the rest per request; ``splits`` is then at most
-    64 - shared.splits (more is cut to that)."""
+    64 - shared.splits (more is cut to that).
+
+    ``meta.max_query_len`` bounds the queries per request, in every replay of a captured
+    step too: capture with the most that a replay will have.  Rows of queries past it come
+    back as NaN and set the status word (``read_status`` = 1)."""
     if shared is not None:
         return _decode_shared(qrot, query, key, value, history, window, meta, layout, scale, splits, rv, output, scratch,
                               store_window, shared)

@@ -412,3 +412,63 @@ def test_rotation_by_rows_columns_and_strides(cuda_lib):
     wide[:, ::2] = b.rv
     b.rv = wide[:, ::2]
     assert torch.equal(b.run(), want)
+
+
+def set_queries(b, query):
+    """New query lengths of the batch's requests in the same device buffers (n unchanged)."""
+    starts = [0]
+    for q in query:
+        starts.append(starts[-1] + q)
+    assert starts[-1] == b.q.shape[0] and len(query) == len(b.seq)
+    tile = b.layout.config.queries_per_tile
+    tasks = [(i, o) for i, q in enumerate(query) for o in range(0, q, tile)]
+    b.meta.query_start_loc.copy_(ints(starts))
+    b.meta.tasks.copy_(ints(tasks + [(-1, -1)] * (b.meta.tasks.shape[0] - len(tasks))))
+    b.meta.task_count.fill_(len(tasks))
+    b.query_lens = list(query)
+
+
+@pytest.mark.parametrize("sharing", [True, False])
+@pytest.mark.parametrize("most", [4, 1, 3])
+def test_replays_follow_new_query_lengths(cuda_lib, sharing, most):
+    """A captured step holds for runs of up to the ``max_query_len`` it was captured with;
+    queries of longer ones come back as NaN with the status word set, never as old scratch."""
+    b = simple(8, 1400, lambda i: 5 * i, 1, 8, 1, seed=22, cfg=make_config(4, 64, mtp=3))
+    b.meta.max_query_len = most
+    plan = kernels.SharedPrefix(8, 8, 8, b.layout, DEV) if sharing else False
+    out = torch.empty(8, 8 * 256, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        if sharing:
+            kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8, shared=plan)
+        b.run(shared=plan, out=out)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for query in ([1] * 8, [4, 4] + [0] * 6, [2, 0, 3, 1, 0, 2, 0, 0], [1] * 8):
+        set_queries(b, query)
+        out.fill_(7.0)
+        kernels.read_status(DEV)
+        graph.replay()
+        past = torch.tensor([i >= most for q in query for i in range(q)], device=DEV)
+        got = out.view(8, 8, 256)
+        assert kernels.read_status(DEV) == (1 if bool(past.any()) else 0)
+        assert bool(torch.isnan(got[past]).all())
+        y, size = b.exact()
+        err, bound = (got.double() - y).abs(), 2**-8 * y.abs() + 1.2 * 2**-8 * size
+        assert bool((err <= bound)[~past].all())
+
+
+def test_partials_of_runs_longer_than_the_launch(cuda_lib):
+    b = simple(2, 300, lambda i: i, 4, 8, 1, seed=23, cfg=make_config(4, 64, mtp=3))
+    whole, lse = kernels.attention_partials(b.q, b.k, b.v, b.history, b.window, b.meta, b.layout, 1 / 16, 1, True)
+    assert kernels.read_status(DEV) == 0
+    b.meta.max_query_len = 2
+    part, short = kernels.attention_partials(b.q, b.k, b.v, b.history, b.window, b.meta, b.layout, 1 / 16, 1, True)
+    assert kernels.read_status(DEV) == 1
+    keep = torch.tensor([0, 1, 4, 5], device=DEV)
+    assert torch.equal(part[keep], whole[keep]) and torch.equal(short[keep], lse[keep])
+    assert bool(torch.isnan(short[keep + 2]).all())
