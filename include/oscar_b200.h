@@ -280,9 +280,9 @@ int64_t oscar_decode_attention_noalloc_max_rows(void);
  * strides) and must not overlap any other row.  q_weight / k_weight: 256 values, fp32
  * (weight_f32) or bf16.  positions: n int64 (positions_64) or int32.  cos_sin: [max_positions,
  * rotary] contiguous, cosines then sines, fp32 (table_f32) or bf16; rotary a multiple of 16,
- * at most 256, 0 for none.  counts (nullable): tokens >= counts[1] are left unwritten.  A
- * token whose position is outside the table is left unwritten and OSCAR_ERR_INVALID goes to
- * *status (nullable). */
+ * at most 256, 0 for none (norms alone: no table, any position).  counts (nullable): tokens
+ * >= counts[1] are left unwritten.  A token whose position is outside the table is left
+ * unwritten and OSCAR_ERR_INVALID goes to *status (nullable). */
 int oscar_qk_norm_rope(const void *query, int64_t qs0, int64_t qs1, const void *key, int64_t ks0, int64_t ks1,
                        int64_t n, int32_t hq, int32_t hkv, const void *q_weight, const void *k_weight,
                        int32_t weight_f32, float weight_offset, float eps, const void *positions,

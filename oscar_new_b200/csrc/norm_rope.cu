@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(32 * kNrWarps, kNrBlocks) qk_norm_rope_kernel(
   float w0[4], w1[4], c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
   load_floats(w0, isq ? P.qw : P.kw, off0, P.weight_f32);
   load_floats(w1, isq ? P.qw : P.kw, off1, P.weight_f32);
-  if (position < 0 || position >= P.max_positions) {  // the token's rows stay unwritten
+  if (P.rotary > 0 && (position < 0 || position >= P.max_positions)) {  // the token's rows stay unwritten
     if (lane == 0 && P.status) atomicExch(P.status, OSCAR_ERR_INVALID);
     return;
   }

@@ -322,8 +322,9 @@ def qk_norm_rope(query, key, q_weight, k_weight, positions, cos_sin, eps=1e-6, w
     of a fused projection); weights [256] and the table cos_sin [positions, rotary]
     (cosines, then sines) fp32 or bf16; positions int64 or int32 [n].
     ``y = x * rsqrt(mean(x^2) + eps) * (w + weight_offset)``, then the first ``rotary`` dims
-    turn: pairs (i, i + rotary/2), or (2i, 2i+1) with ``interleaved``.  fp32 inside (a row's
-    sum of squares has to fit: elements up to about 2^59).
+    turn: pairs (i, i + rotary/2), or (2i, 2i+1) with ``interleaved``; none for a table of
+    no columns, whatever the positions.  fp32 inside (a row's sum of squares has to fit:
+    elements up to about 2^59).
     Outputs are new tensors, or ``query_out`` / ``key_out``: an output may be its own input,
     and must otherwise not overlap the other rows.  ``counts`` (device [requests, active
     tokens]) leaves the tokens behind the active ones as they were.  A token whose position

@@ -172,3 +172,20 @@ def test_strided_counts(cuda_lib):
     counts = torch.tensor([2, 6, 3, 6], dtype=torch.int32, device=DEV)[::2]  # 3 active tokens
     kernels.qk_norm_rope(q, k, w, w, pos, tab, counts=counts, query_out=qo, key_out=ko)
     assert bool((qo[3:] == 7).all()) and not bool((qo[2] == 7).any())
+
+
+@pytest.mark.parametrize("rows", [0, 3])
+def test_no_rotation_takes_any_position(cuda_lib, rows):
+    """rotary 0: norms alone, no table row is looked up."""
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(7, 4, 256, generator=g).bfloat16().to(DEV)
+    k = torch.randn(7, 2, 256, generator=g).bfloat16().to(DEV)
+    w, tab = torch.randn(256, generator=g).to(DEV), torch.zeros(rows, 0, device=DEV)
+    pos = torch.tensor([0, 2, 3, -1, 1 << 40, 5, 1], device=DEV)
+    kernels.read_status(DEV)
+    for interleaved in (False, True):
+        qo, ko = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+        kernels.qk_norm_rope(q, k, w, w, pos, tab, interleaved=interleaved, query_out=qo, key_out=ko)
+        assert kernels.read_status(DEV) == 0
+        check(qo, formula(q, w, 0.0, 1e-6, tab, 0, interleaved))
+        check(ko, formula(k, w, 0.0, 1e-6, tab, 0, interleaved))
