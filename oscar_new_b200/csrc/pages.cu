@@ -473,6 +473,7 @@ int launch_copies(const Pool &p, const oscar_geometry &geo, void *history, void 
   C.slices_w = (C.window_bytes + kSliceBytes - 1) / kSliceBytes;
   C.parents = parents, C.children = children, C.rows = rows, C.marked = marked;
   const int64_t units = std::max<int64_t>(jobs * (C.slices_h + C.slices_w), rows);
+  if (units == 0) return OSCAR_OK;  // a pool of one page has none to move
   const int grid = (int)std::min<int64_t>(units, 148 * 8);
   copy_pages_kernel<<<grid, kCopyThreads, 0, st>>>(C);
   OSCAR_CHECK_LAUNCH();

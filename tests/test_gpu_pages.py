@@ -159,3 +159,17 @@ def test_caches_of_several_layers_repeat_a_call_from_one_state(cuda_lib):
         assert torch.equal(layers[0][1].view(torch.int16), layers[1][1].view(torch.int16))
         kernels.resize_requests(p.pool, p.ints([0]), p.ints([0]))  # holes for the second call
     assert not torch.equal(layers[0][0], p.history)
+
+
+@pytest.mark.parametrize("pages", [1, 2, 3])
+def test_pools_of_very_few_pages(cuda_lib, pages):
+    layout = CacheLayout(256, kv_heads=1, config=make_config(4, 64))
+    p = Pair(pages, 3, 512, layout)
+    p.compact()  # nothing lives
+    p.resize([1, 0], [200, 300])
+    p.compact()
+    p.resize([1], [0])
+    p.compact()
+    p.resize([2, 0], [100, 512])
+    p.fork([2, 2], [0, 1])
+    p.compact()
