@@ -14,7 +14,7 @@
 //   y_a = r (x_a (w_a cos) - x_b (w_b sin)),  y_b = r (x_b (w_b cos) + x_a (w_a sin)).
 // The first rows are asked for before the position is known.
 //
-// Measured on a B200: 16384 tokens, 24 + 4 heads, 64 rotary dims, bf16 (475 MB): 90 us, 5.2
+// Measured on a B200: 16384 tokens, 24 + 4 heads, 64 rotary dims, bf16 (475 MB): 91 us, 5.2
 // TB/s; with one 16-byte load a lane and the partner of a pair shuffled in, 122 us.
 #include <algorithm>
 
@@ -24,7 +24,7 @@ namespace oscar {
 namespace {
 
 constexpr int kNrWarps = 8, kNrBlocks = 4;  // 32 warps per SM
-constexpr int kNrRows = 2;                  // rows in flight per warp (4: 112 us, 1: 111)
+constexpr int kNrRows = 2;                  // rows in flight per warp (1: 109 us, 4: 109 us and spills)
 
 struct NrParams {
   const __nv_bfloat16 *q, *k;
@@ -133,6 +133,15 @@ __global__ void __launch_bounds__(32 * kNrWarps, kNrBlocks) qk_norm_rope_kernel(
             y1[2 * e - 4] = ya, y1[2 * e - 3] = yb;
         } else {
           y0[e] = ya, y1[e] = yb;
+        }
+      }
+      // Dims that do not turn met their lane partner with coefficient 0, and an infinite one
+      // (r = 0 then) made NaN of them: without it, in rows that hold one (90.3 -> 91.2 us).
+      if (!(ss < INFINITY) && !turns) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y0[e] = r * (x0[e] * (INTERLEAVED ? (e & 1 ? bb[e >> 1] : aa[e >> 1]) : aa[e]));
+          y1[e] = r * (x1[e] * (INTERLEAVED ? (e & 1 ? bb[2 + (e >> 1)] : aa[2 + (e >> 1)]) : bb[e]));
         }
       }
       *reinterpret_cast<uint2 *>(dst + i * o1 + off0) = make_uint2(pack_bf162(y0[0], y0[1]), pack_bf162(y0[2], y0[3]));

@@ -189,3 +189,22 @@ def test_no_rotation_takes_any_position(cuda_lib, rows):
         assert kernels.read_status(DEV) == 0
         check(qo, formula(q, w, 0.0, 1e-6, tab, 0, interleaved))
         check(ko, formula(k, w, 0.0, 1e-6, tab, 0, interleaved))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+def test_infinities_reach_what_the_formula_says(cuda_lib, interleaved, value):
+    """An infinity makes the row's scale 0: its own dim is NaN, and the partner it turns with;
+    dims that do not turn have no partner."""
+    rotary, g = 64, torch.Generator().manual_seed(7)
+    at = [0, 5, 37, 63, 64, 68, 100, 131, 200, 255]
+    q = torch.randn(len(at), 3, 256, generator=g).bfloat16()
+    for t, d in enumerate(at):
+        q[t, 1, d] = value
+    q = q.to(DEV)
+    w, tab, pos = torch.randn(256, generator=g).to(DEV), table(40, rotary), torch.arange(1, len(at) + 1, device=DEV)
+    qo, ko = kernels.qk_norm_rope(q, q[:, 1:2], w, w, pos, tab, interleaved=interleaved)
+    check(qo, formula(q, w, 0.0, 1e-6, tab[pos], rotary, interleaved))
+    check(ko, formula(q[:, 1:2], w, 0.0, 1e-6, tab[pos], rotary, interleaved))
+    for t, d in enumerate(at):
+        assert int(torch.isnan(qo[t, 1]).sum()) == (2 if d < rotary else 1)
