@@ -359,7 +359,8 @@ int oscar_resize_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, i
 
 /* Move the live pages onto the page numbers 1 .. live: the k-th live page above goes to the
  * k-th free page within.  Slots that some row uses move, and the window of a row's first
- * page; counts and table follow, table entries past a row's pages become 0.
+ * page; a page that no row holds, only its count, moves with all its slots and window.
+ * Counts and table follow, table entries past a row's pages become 0.
  * summary[0..1] = {live pages, moved pages}; moved_to[num_pages] = each page's new number,
  * -1 for a page that was free. */
 int oscar_compact_pages(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, void *history,

@@ -240,7 +240,11 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const CopyPara
     PageJob job = p.jobs[u / per_job];
     const int s = (int)(u % per_job);
     if (!page_ok(p, job.src) || !page_ok(p, job.dst)) continue;
-    if (C.marked) job.tokens = p.used[job.src], job.window = p.list[job.src];
+    if (C.marked) {
+      job.tokens = p.used[job.src], job.window = p.list[job.src];
+      // no row holds it, its count alone does: what it keeps is not known here
+      if (job.tokens == 0) job.tokens = p.block_tokens, job.window = 1;
+    }
     const bool hist = s < C.slices_h;
     const int64_t at = (int64_t)(hist ? s : s - C.slices_h) * kSliceBytes;
     const int64_t bytes = hist ? (int64_t)job.tokens * C.slot_row : (job.window ? C.window_bytes : 0);
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Pool p
   }
 }
 
-// used[page] = most tokens a request keeps in a page, list[page] = 1 when a request starts
+// used[page] = most tokens a request keeps in a page (0: no request does), list[page] = 1 when a request starts
 // in it (its window), both by the old page numbers; the table's blocks follow their pages
 __global__ void __launch_bounds__(kCopyThreads) compact_rows_kernel(const Pool p) {
   const int r = blockIdx.x;

@@ -436,8 +436,9 @@ def resize_requests(pool, rows, lens):
 
 def compact_pages(pool, history, window):
     """Move a pool's live pages onto the lowest page numbers (1 .. live), with the slots and
-    windows they hold; counts and table follow.  Returns (summary int32 [live pages, moved
-    pages], moved_to int32 [num_pages]: each page's new number, -1 for a free page)."""
+    windows they hold (all of them, for a page that only its count holds); counts and table
+    follow.  Returns (summary int32 [live pages, moved pages], moved_to int32 [num_pages]:
+    each page's new number, -1 for a free page)."""
     pool.check_stripes(history, window)
     device = _same_device(pool.arena, history, window)
     summary, moved_to = pool.arena.new_empty(2), pool.arena.new_empty(pool.num_pages)

@@ -8,7 +8,9 @@ length in tokens of every request row, the block table the attention kernels rea
 * a row of ``L`` tokens holds ``ceil(L / block_tokens)`` pages, in order, its first page
   owning the request's BF16 window; table entries past them are 0;
 * full pages may be shared between rows (their count is the number of rows that hold
-  them); a row's first page and its partial last page are its own;
+  them); a row's first page and its partial last page are its own.  A host may raise the
+  counts of a row's pages by one to keep them when the row is released (a prompt to come
+  back to): compaction takes such pages along whole and ``moved_to`` says where;
 * fresh pages are the free pages of the lowest numbers.
 
 ``kernels.resize_requests`` admits, grows and releases rows, ``kernels.fork_requests``

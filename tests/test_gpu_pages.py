@@ -173,3 +173,22 @@ def test_pools_of_very_few_pages(cuda_lib, pages):
     p.resize([2, 0], [100, 512])
     p.fork([2, 2], [0, 1])
     p.compact()
+
+
+def test_compaction_takes_pages_along_that_only_a_count_holds(cuda_lib):
+    """A host that keeps a prompt's pages by their counts alone (no row) finds the whole pages,
+    slots and windows, at their new numbers."""
+    layout = CacheLayout(256, kv_heads=2, config=make_config(4, 64))
+    p = Pair(20, 5, 2048, layout, seed=4)
+    p.resize([0, 1, 2], [1000, 700, 300])
+    kept = p.model.pages[1]
+    p.pool.refcounts[kept] += 1
+    kernels.resize_requests(p.pool, p.ints([1, 0]), p.ints([0, 0]))
+    before = p.history.view(20, -1)[kept].clone(), p.window.view(20, -1)[kept].clone().view(torch.int16)
+    summary, to = kernels.compact_pages(p.pool, p.history, p.window)
+    assert summary.tolist() == [5, 5 - len([x for x in kept if x <= 5])] and p.pool.refcounts.tolist() == [1] * 6 + [0] * 14
+    now = to[kept].long()
+    hist, win = p.history.view(20, -1)[now], p.window.view(20, -1)[now].view(torch.int16)
+    size = layout.history_page_bytes
+    assert torch.equal(hist[:, :size], before[0][:, :size])
+    assert torch.equal(win[:, :layout.window_page_bytes // 2], before[1][:, :layout.window_page_bytes // 2])
