@@ -334,7 +334,7 @@ int oscar_decode_attention_shared(const void *qrot, const void *query, int64_t q
  * 128-token kernel blocks (unused entries 0), then workspace that the calls below share,
  * so calls on one arena must be ordered.  A row of L tokens holds ceil(L / block_tokens)
  * pages; fresh pages are the free pages of the lowest numbers, handed out in list order:
- * results depend on the state and the list alone.  Writes the word offsets {counts,
+ * results depend on the state and the list alone.  max_reqs * columns < 2^31.  Writes the word offsets {counts,
  * lengths, table, end of the state, total words} to offsets[0..4]. */
 int oscar_page_pool_layout(int32_t num_pages, int32_t max_reqs, int32_t columns, int64_t *offsets);
 

@@ -42,7 +42,7 @@ int64_t up4(int64_t x) { return (x + 3) / 4 * 4; }
 
 bool pool_offsets(int64_t num_pages, int64_t max_reqs, int64_t columns, int64_t (&off)[10]) {
   if (num_pages < 1 || max_reqs < 1 || columns < 1 || num_pages > (1 << 24) || max_reqs > (1 << 20) ||
-      columns > (1 << 24) || max_reqs * columns > ((int64_t)1 << 31))
+      columns > (1 << 24) || max_reqs * columns > INT32_MAX)  // sums of pages over all rows are int32
     return false;
   const int64_t jobs = std::max(2 * max_reqs, num_pages);
   off[0] = 0;                                   // reference counts
@@ -71,7 +71,10 @@ bool make_pool(Pool &p, int32_t *arena, int32_t num_pages, int32_t max_reqs, int
   return true;
 }
 
-OSCAR_DEVINL int pages_of(const Pool &p, int tokens) { return (tokens + p.block_tokens - 1) / p.block_tokens; }
+// unsigned: tokens (not negative) may be up to 2^31 - 1
+OSCAR_DEVINL int pages_of(const Pool &p, int tokens) {
+  return (int)(((uint32_t)tokens + p.block_tokens - 1) / (uint32_t)p.block_tokens);
+}
 // tokens a table row can hold
 OSCAR_DEVINL int64_t row_tokens(const Pool &p) { return (int64_t)(p.columns / p.per_page) * p.block_tokens; }
 OSCAR_DEVINL int table_page(const Pool &p, int row, int page) {

@@ -192,3 +192,13 @@ def test_compaction_takes_pages_along_that_only_a_count_holds(cuda_lib):
     size = layout.history_page_bytes
     assert torch.equal(hist[:, :size], before[0][:, :size])
     assert torch.equal(win[:, :layout.window_page_bytes // 2], before[1][:, :layout.window_page_bytes // 2])
+
+
+def test_rows_of_nearly_two_to_the_31_tokens(cuda_lib):
+    layout = CacheLayout(1 << 21, kv_heads=1, config=make_config(4, 64))
+    pool, model = PagePool(1100, 1, 1 << 24, layout, DEV), PoolModel(1100, 1, 1 << 24, layout)
+    i = lambda x: torch.tensor([x], dtype=torch.int32, device=DEV)  # noqa: E731
+    for tokens in (2**31 - 1 - 2**21, 2**31 - 1, 0):
+        assert kernels.resize_requests(pool, i(0), i(tokens)).tolist() == model.resize([0], [tokens])
+        assert pool.seq_lens.tolist() == model.lens and pool.refcounts.tolist() == model.refs
+        assert np.array_equal(pool.block_tables.cpu().numpy(), model.table())

@@ -102,3 +102,10 @@ def test_model_keeps_its_own_rules():
         assert counts[1:] == m.refs[1:]
         for row, n in zip(m.pages, m.lens):  # first and partial last pages are private
             assert not row or m.refs[row[0]] == 1 and (n % 768 == 0 or m.refs[row[-1]] == 1)
+
+
+def test_tables_whose_pages_pass_32_bits_are_refused():
+    off = torch.zeros(5, dtype=torch.int64)
+    layout = _lib.lib().oscar_page_pool_layout
+    assert layout(4, 1 << 20, 2047, off.data_ptr()) == 0 and layout(4, 127, 1 << 24, off.data_ptr()) == 0
+    assert layout(4, 1 << 20, 2048, off.data_ptr()) == 1 and layout(4, 128, 1 << 24, off.data_ptr()) == 1
