@@ -612,8 +612,12 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
         raise ValueError("the plan was made for other heads, another layout or fewer requests")
     elif reqs < shared.max_reqs:
         raise ValueError(f"groups and prefix_lens must have the plan's {shared.max_reqs} entries")
+    for name in ("query_start_loc", "seq_lens", "counts"):
+        t = getattr(meta, name)
+        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector, got {tuple(t.shape)} {t.dtype}")
     table = meta.block_tables
-    device = _same_device(groups, prefix_lens, shared.plan, meta.counts, table)
+    device = _same_device(groups, prefix_lens, shared.plan, meta.query_start_loc, meta.seq_lens, meta.counts, table)
     groups, prefix_lens = _dense(groups), _dense(prefix_lens)
     with device:
         _lib.call("oscar_prepare_shared_prefix", meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),
@@ -643,6 +647,7 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
     if table.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
     device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan, table,
+                          meta.query_start_loc, meta.seq_lens, meta.counts, meta.tasks, meta.task_count,
                           None if scratch is None else scratch.partials)
     if n == 0:
         return output

@@ -472,3 +472,18 @@ def test_partials_of_runs_longer_than_the_launch(cuda_lib):
     keep = torch.tensor([0, 1, 4, 5], device=DEV)
     assert torch.equal(part[keep], whole[keep]) and torch.equal(short[keep], lse[keep])
     assert bool(torch.isnan(short[keep + 2]).all())
+
+
+@pytest.mark.parametrize("name", ["query_start_loc", "seq_lens", "counts", "tasks", "task_count", "block_tables"])
+def test_metadata_on_the_host_is_refused(cuda_lib, name):
+    b = simple(4, 500, lambda i: i, 1, 8, 1, seed=26)
+    b.run()
+    kept, here = b.plan, getattr(b.meta, name)
+    setattr(b.meta, name, here.cpu())
+    with pytest.raises(RuntimeError, match="CUDA device only"):
+        b.run(shared=kept)
+    if name in ("query_start_loc", "seq_lens", "counts", "block_tables"):
+        with pytest.raises(RuntimeError, match="CUDA device only"):
+            kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8)
+    setattr(b.meta, name, here)
+    b.check(b.run())

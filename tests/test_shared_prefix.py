@@ -113,3 +113,13 @@ def test_c_entries_refuse_before_any_launch():
                 dict(qrot=p + 8), dict(qs0=6140), dict(hist=None), dict(part=None), dict(out=p + 2), dict(wp=-1)):
         assert call(**bad) == 1, bad
     assert call(n=0) == 0
+
+
+@pytest.mark.parametrize("name", ["query_start_loc", "seq_lens", "counts"])
+def test_metadata_that_the_plan_would_misread_is_refused(name):
+    ok = torch.zeros(3, dtype=torch.int32)
+    for bad in (lambda t: t.long(), lambda t: torch.stack((t, t), 1)[:, 0], lambda t: t[None]):
+        m = meta()
+        setattr(m, name, bad(getattr(m, name)))
+        with pytest.raises(ValueError, match=name):
+            kernels.prepare_shared_prefix(m, ok, ok, LAYOUT, 24)
