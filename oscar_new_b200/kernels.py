@@ -607,7 +607,7 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
         raise ValueError("groups and prefix_lens must be int32 with an entry per request")
     if shared is None:
         tokens = getattr(meta, "num_actual_tokens", None) or meta.num_reqs * max(1, meta.max_query_len)
-        shared = SharedPrefix(reqs, tokens, hq, layout, groups.device, _blank=False)
+        shared = SharedPrefix(max(reqs, 1), tokens, hq, layout, groups.device, _blank=reqs == 0)
     elif shared.hq != hq or shared.max_reqs < meta.num_reqs or shared.layout != layout:
         raise ValueError("the plan was made for other heads, another layout or fewer requests")
     elif reqs < shared.max_reqs:
@@ -618,6 +618,8 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
             raise ValueError(f"{name} must be a contiguous int32 vector, got {tuple(t.shape)} {t.dtype}")
     table = meta.block_tables
     device = _same_device(groups, prefix_lens, shared.plan, meta.query_start_loc, meta.seq_lens, meta.counts, table)
+    if reqs == 0:  # a new plan of an empty step: it shares nothing as it is
+        return shared
     groups, prefix_lens = _dense(groups), _dense(prefix_lens)
     with device:
         _lib.call("oscar_prepare_shared_prefix", meta.query_start_loc.data_ptr(), meta.seq_lens.data_ptr(),

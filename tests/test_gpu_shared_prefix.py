@@ -487,3 +487,16 @@ def test_metadata_on_the_host_is_refused(cuda_lib, name):
             kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8)
     setattr(b.meta, name, here)
     b.check(b.run())
+
+
+def test_step_without_requests(cuda_lib):
+    b = simple(4, 500, lambda i: i, 1, 8, 1, seed=27)
+    empty = ints([])
+    b.meta.num_reqs = b.meta.max_query_len = 0
+    b.meta.counts.zero_()
+    b.meta.task_count.zero_()
+    plan = kernels.prepare_shared_prefix(b.meta, empty, empty, b.layout, 8)
+    for name in ("qrot", "q", "k", "v"):
+        setattr(b, name, getattr(b, name)[:0])
+    assert b.run(shared=plan).shape == (0, 8, 256)
+    assert kernels.read_status(DEV) == 0
