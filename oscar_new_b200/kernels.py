@@ -579,13 +579,15 @@ class SharedPrefix:
         self.max_reqs, self.max_tokens, self.splits, self.hq, self.layout = max_reqs, max_tokens, splits, hq, layout
         # a plan that was never filled shares nothing
         self.plan = (torch.zeros if _blank else torch.empty)(words, dtype=torch.int32, device=device)
-        self._geometry = None
+        self._geometries: dict = {}
 
     def geometry(self, table_stride: int, query_tile: int):
-        geo = self._geometry
-        if geo is None or geo.table_stride != table_stride:
-            geo = self._geometry = geometry(self.layout, self.hq, table_stride)
-        geo.query_tile = query_tile
+        # one struct per form, never changed: threads may call with the same plan
+        geo = self._geometries.get((table_stride, query_tile))
+        if geo is None:
+            geo = geometry(self.layout, self.hq, table_stride)
+            geo.query_tile = query_tile
+            self._geometries[table_stride, query_tile] = geo
         return geo
 
 

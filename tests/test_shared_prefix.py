@@ -123,3 +123,10 @@ def test_metadata_that_the_plan_would_misread_is_refused(name):
         setattr(m, name, bad(getattr(m, name)))
         with pytest.raises(ValueError, match=name):
             kernels.prepare_shared_prefix(m, ok, ok, LAYOUT, 24)
+
+
+def test_a_plan_used_by_two_callers_keeps_their_geometries_apart():
+    plan = kernels.SharedPrefix(3, 3, 24, LAYOUT, "cpu")
+    four, one, wide = plan.geometry(12, 4), plan.geometry(12, 1), plan.geometry(24, 4)
+    assert (four.query_tile, one.query_tile, wide.query_tile) == (4, 1, 4)
+    assert (four.table_stride, one.table_stride, wide.table_stride) == (12, 12, 24)
