@@ -639,8 +639,10 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
         raise ValueError("the plan was made for other heads, another layout or fewer requests")
     if not scale > 0:
         raise ValueError("a shared prefix needs a positive softmax scale")
-    if history.numel() % layout.stripe_page_bytes or not history.is_contiguous():
-        raise ValueError("the history view must be whole contiguous pages")
+    if history.dtype != torch.uint8 or history.numel() % layout.stripe_page_bytes or not history.is_contiguous():
+        raise ValueError("the history view must be whole contiguous pages of bytes")
+    if window.dtype != torch.bfloat16 or not window.is_contiguous() or 2 * window.numel() < history.numel():
+        raise ValueError("the window view must be the contiguous bf16 stripe beside the history")
     if output.dtype != torch.bfloat16 or not output.is_contiguous() or output.numel() != query.numel():
         raise ValueError("output must be contiguous bf16 [n, Hq * 256]")
     if qrot.shape != query.shape or qrot.dtype != torch.bfloat16 or rv.shape != (256, 256) or rv.dtype != torch.bfloat16:

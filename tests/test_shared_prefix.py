@@ -130,3 +130,16 @@ def test_a_plan_used_by_two_callers_keeps_their_geometries_apart():
     four, one, wide = plan.geometry(12, 4), plan.geometry(12, 1), plan.geometry(24, 4)
     assert (four.query_tile, one.query_tile, wide.query_tile) == (4, 1, 4)
     assert (four.table_stride, one.table_stride, wide.table_stride) == (12, 12, 24)
+
+
+@pytest.mark.parametrize("window", [
+    torch.zeros(LAYOUT.stripe_page_bytes - 8, dtype=torch.bfloat16), torch.zeros(LAYOUT.stripe_page_bytes, dtype=torch.float16),
+    torch.zeros(2 * LAYOUT.stripe_page_bytes, dtype=torch.bfloat16)[::2]])
+def test_windows_other_than_the_caches_are_refused(window):
+    with pytest.raises(ValueError, match="window view"):
+        kernels.decode_attention(**{**decode_args(), "window": window})
+
+
+def test_a_history_of_another_type_is_refused():
+    with pytest.raises(ValueError, match="whole contiguous pages"):
+        kernels.decode_attention(**{**decode_args(), "history": torch.zeros(LAYOUT.stripe_page_bytes, dtype=torch.bfloat16)})
