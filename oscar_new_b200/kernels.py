@@ -352,7 +352,9 @@ def qk_norm_rope(query, key, q_weight, k_weight, positions, cos_sin, eps=1e-6, w
     counts = None if counts is None else _dense(counts)
     qo, ko = _output_rows(query_out, query), _output_rows(key_out, key)
     if query_out is not None or key_out is not None:
-        same = [o.data_ptr() == i.data_ptr() and o.stride() == i.stride() for o, i in ((qo, query), (ko, key))]
+        # the same rows: strides of dims of one element do not matter
+        same = [o.data_ptr() == i.data_ptr() and all(a == b for a, b, size in zip(o.stride(), i.stride(), o.shape) if size > 1)
+                for o, i in ((qo, query), (ko, key))]
         pairs = [(qo, ko), (qo, key), (ko, query)] + [p for p, s in zip(((qo, query), (ko, key)), same) if not s]
         if not all(0 in a.shape or 0 in b.shape or _rows_apart(a, b) for a, b in pairs):
             raise ValueError("an output overlaps rows other than its own input's")

@@ -82,3 +82,16 @@ def test_c_entry_refuses_before_any_launch():
                 dict(q=p + 2), dict(ko=p + 8), dict(qs0=1020), dict(kos1=4), dict(mp=-1), dict(tab=p + 4)):
         assert call(**bad) == 1, bad
     assert call(n=0) == 0
+
+
+def test_one_token_in_place_under_another_stride():
+    """A dim of one element has no stride that matters: the rows are the input's own."""
+    fused = torch.zeros(2, 6 * 256, dtype=torch.bfloat16)
+    flat, a = fused.view(-1), args(n=1)
+    a["query"], a["key"] = fused[:, :1024].unflatten(1, (4, 256))[:1], fused[:, 1024:].unflatten(1, (2, 256))[:1]
+    q, k = flat[:1024].view(1, 4, 256), flat[1024:1536].view(1, 2, 256)
+    assert q.stride() != a["query"].stride() and k.stride() != a["key"].stride()
+    with pytest.raises(RuntimeError, match="CUDA device only"):
+        kernels.qk_norm_rope(**a, query_out=q, key_out=k)
+    with pytest.raises(ValueError, match="overlaps rows"):
+        kernels.qk_norm_rope(**a, query_out=q, key_out=flat[512:1024].view(1, 2, 256))
