@@ -216,7 +216,8 @@ int oscar_merge_paths(const void *a, const float *la, const float *b, int64_t b_
                       const int32_t *counts, void *out, void *stream);
 
 /* Write current BF16 K/V into each request's sink/ring window (latest writer per
- * ring slot).  num_programs = min(n, max_reqs) as in reference kernels.py:598-620. */
+ * ring slot).  num_programs = min(n, max_reqs) as in reference kernels.py:598-620; requests
+ * past it (a step may have more of them than tokens) are stored too. */
 int oscar_store_windows(const void *key, int64_t ks0, int64_t ks1, const void *value,
                         int64_t vs0, int64_t vs1, void *window, const int32_t *qstarts,
                         const int32_t *seq_lens, const int32_t *table, const int32_t *counts,

@@ -920,15 +920,15 @@ __global__ void __launch_bounds__(kFinThreads) finalize_kernel(FinalParams P) {
 }
 
 // ----------------------------------------------------------------------------
-// window store (reference _window_store_kernel): CTA per request, warp per
-// (window index, head) pair, 16-byte lanes.
+// window store (reference _window_store_kernel): CTA per request (and the requests a grid
+// further, when a step has more requests than tokens), warp per (window index, head) pair,
+// 16-byte lanes.
 // ----------------------------------------------------------------------------
 OSCAR_DEVINL void store_window(int req, int warps, const __nv_bfloat16 *__restrict__ key, int64_t ks0, int64_t ks1,
                                const __nv_bfloat16 *__restrict__ value, int64_t vs0, int64_t vs1,
                                __nv_bfloat16 *__restrict__ window, const int32_t *__restrict__ qstarts,
                                const int32_t *__restrict__ seq_lens, const int32_t *__restrict__ table,
                                const int32_t *__restrict__ counts, const oscar_geometry &g) {
-  if (req >= counts[0]) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int qstart = qstarts[req];
   const int qend = min(qstarts[req + 1], counts[1]);
@@ -968,7 +968,8 @@ __global__ void __launch_bounds__(256) window_store_kernel(const __nv_bfloat16 *
                                                            const int32_t *__restrict__ table,
                                                            const int32_t *__restrict__ counts,
                                                            oscar_geometry g) {
-  store_window(blockIdx.x, 8, key, ks0, ks1, value, vs0, vs1, window, qstarts, seq_lens, table, counts, g);
+  for (int req = blockIdx.x; req < counts[0]; req += gridDim.x)
+    store_window(req, 8, key, ks0, ks1, value, vs0, vs1, window, qstarts, seq_lens, table, counts, g);
 }
 
 // ----------------------------------------------------------------------------
@@ -994,8 +995,9 @@ struct WindowParams {
 __global__ void __launch_bounds__(kFinWideThreads, 1) finalize_wide_kernel(FinalParams P, WindowParams W, int row_blocks) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   if (blockIdx.x >= row_blocks) {
-    store_window(blockIdx.x - row_blocks, kFinWideRows, W.key, W.ks0, W.ks1, W.value, W.vs0, W.vs1, W.window, W.qstarts,
-                 W.seq_lens, W.table, P.counts, W.geo);
+    for (int req = blockIdx.x - row_blocks; req < P.counts[0]; req += gridDim.x - row_blocks)
+      store_window(req, kFinWideRows, W.key, W.ks0, W.ks1, W.value, W.vs0, W.vs1, W.window, W.qstarts, W.seq_lens, W.table,
+                   P.counts, W.geo);
     return;
   }
   __nv_bfloat16 *sB = reinterpret_cast<__nv_bfloat16 *>(smem_raw);  // [256 n][256 k], chunks ^ (n & 7)

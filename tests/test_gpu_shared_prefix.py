@@ -500,3 +500,20 @@ def test_step_without_requests(cuda_lib):
         setattr(b, name, getattr(b, name)[:0])
     assert b.run(shared=plan).shape == (0, 8, 256)
     assert kernels.read_status(DEV) == 0
+
+
+@pytest.mark.parametrize("sharing", [True, False])
+def test_windows_of_requests_behind_many_without_tokens(cuda_lib, sharing):
+    """More requests than tokens: the windows of the last ones are stored too."""
+    query = [0] * 9 + [1, 0, 2]
+    b = Batch([0] * 12, [500] * 12, [600 + i for i in range(12)], query, 8, 1, make_config(4, 64, mtp=3), seed=25)
+    before = b.win.clone()
+    b.run(shared=sharing, store_window=True)
+    torch.cuda.synchronize()
+    want, t = before.clone(), 0
+    for i, q in enumerate(query):
+        for pos in range(b.seq[i] - q, b.seq[i]):
+            at = pos if pos < 4 else 4 + pos % b.layout.config.ring_tokens
+            want[b.rows[i][0], at, 0], want[b.rows[i][0], at, 1] = b.k[t], b.v[t]
+            t += 1
+    assert torch.equal(b.win.view(torch.int16), want.view(torch.int16))
