@@ -202,3 +202,23 @@ def test_rows_of_nearly_two_to_the_31_tokens(cuda_lib):
         assert kernels.resize_requests(pool, i(0), i(tokens)).tolist() == model.resize([0], [tokens])
         assert pool.seq_lens.tolist() == model.lens and pool.refcounts.tolist() == model.refs
         assert np.array_equal(pool.block_tables.cpu().numpy(), model.table())
+
+
+@pytest.mark.parametrize("block,columns,pages", [(128, 300, 900), (384, 600, 500)])
+def test_long_rows(cuda_lib, block, columns, pages):
+    """Rows of more pages than a warp has lanes and of more table words than a block has
+    threads, through every operator."""
+    layout = CacheLayout(block, kv_heads=1, config=make_config(0, 16))
+    p, rng = Pair(pages, 7, columns * 128, layout, seed=columns), random.Random(columns)
+    long = columns * 128
+    p.resize([0, 1, 2], [long, long - 129, 40 * block + 1])
+    p.fork([0, 1, 1], [3, 4, 5])
+    p.resize([1, 0, 6, 2], [0, 0, long // 2, 70 * block])
+    p.compact()
+    p.fork([3, 6, 2], [0, 1, 1])
+    for _ in range(8):
+        rows = rng.sample(range(7), 4)
+        p.resize(rows, [rng.choice([0, rng.randint(1, long), long]) for _ in rows])
+        p.fork([rng.randint(0, 6) for _ in range(3)], [rng.randint(0, 6) for _ in range(3)])
+        if rng.random() < 0.5:
+            p.compact()

@@ -517,3 +517,43 @@ def test_windows_of_requests_behind_many_without_tokens(cuda_lib, sharing):
             want[b.rows[i][0], at, 0], want[b.rows[i][0], at, 1] = b.k[t], b.v[t]
             t += 1
     assert torch.equal(b.win.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("max_reqs", [300, 2100])
+def test_more_requests_than_the_plan_kernel_has_threads(cuda_lib, max_reqs):
+    """Groups on both sides of the 256th request; at 2100 requests the plan kernel needs more
+    than the default 48 KB of shared memory."""
+    labels = [0] * 100 + [1] * 90 + [-1] * 30 + [2] * 60 + [3] * 20
+    prefix = [300] * 100 + [200] * 90 + [0] * 30 + [500] * 60 + [150] * 20
+    seq = [p + 80 + i % 7 for i, p in enumerate(prefix)]
+    b = Batch(labels, prefix, seq, [1] * 300, 6, 1, make_config(4, 64), block=256, seed=24, max_reqs=max_reqs)
+    b.check(b.run(splits=4))
+    items, ends, used = b.plan_words()
+    assert ends[:300] == prefix and not any(ends[300:]) and not any(used[300:])
+    rows = {it[0]: 0 for it in items}
+    assert sorted(rows) == [0, 100, 220, 280]
+    spans = sorted((it[0], it[1], it[4], it[5]) for it in items)
+    for tok0, members, p in ((0, 100, 300), (100, 90, 200), (220, 60, 500), (280, 20, 150)):
+        for row0 in range(0, 6 * members, 128):
+            mine = [s[2:] for s in spans if s[:2] == (tok0, row0)]
+            assert mine[0][0] == 0 and mine[-1][1] == -(-p // 64) and all(x[1] == y[0] for x, y in zip(mine, mine[1:]))
+    assert len({(it[0], it[1], it[7]) for it in items}) == len(items)
+
+
+def test_plan_of_the_most_requests(cuda_lib):
+    """8192 requests, the plan's limit: pairs of them share, one token each."""
+    n = 8192
+    lay = CacheLayout(256, kv_heads=1, config=make_config(4, 64))
+    meta = SimpleNamespace(query_start_loc=torch.arange(n + 1, dtype=torch.int32, device=DEV),
+                           seq_lens=torch.full((n,), 400, dtype=torch.int32, device=DEV),
+                           block_tables=torch.zeros(n, 4, dtype=torch.int32, device=DEV), counts=ints([n, n]), num_reqs=n,
+                           max_num_reqs=n, max_query_len=1)
+    groups, lens = torch.arange(n, dtype=torch.int32, device=DEV) // 2, ints([130] * n)
+    plan = kernels.prepare_shared_prefix(meta, groups, lens, lay, 6)
+    words = plan.plan.cpu()
+    items = words[8 + 2 * n:8 + 2 * n + 8 * int(words[0])].view(-1, 8)
+    assert int(words[0]) >= n // 2 and bool((words[8:8 + n] == 130).all())
+    used = words[8 + n:8 + 2 * n]
+    assert torch.equal(torch.bincount(items[:, 0].long() // 2, minlength=n // 2), used[::2].long())
+    assert torch.equal(used[::2], used[1::2]) and bool((items[:, 2] == 12).all()) and bool((items[:, 6] == 130).all())
+    assert torch.equal(items[:, 3], items[:, 0])
