@@ -406,7 +406,9 @@ def fork_requests(pool, parents, children, history, window):
     partial last page's used slots are copied to fresh pages of the cache (``history`` /
     ``window``, the flat views of ``CacheLayout.tensor_views``).  Returns int32 [count]: 1
     forked; 0 the free pages ran out at this pair or before; -1 not a valid pair (an empty
-    or unknown parent, a child that holds tokens or that an earlier pair names)."""
+    or unknown parent, a child that holds tokens or that an earlier pair names).  A parent
+    whose last tokens were rejected drafts waits until ``kept >= length // block_tokens *
+    block_tokens`` (``pages``)."""
     pool.check_stripes(history, window)
     parents, children = _pool_list(pool, parents, children)
     device = _same_device(pool.arena, parents, children, history, window)
@@ -425,7 +427,7 @@ def resize_requests(pool, rows, lens):
     Releases come before growth, so their pages serve the same call.  Returns int32
     [count]: 1 done; 0 the free pages ran out at this entry or before (the row is
     unchanged); -1 refused (row or length out of range, a shorter length other than 0, a
-    row that an earlier entry names)."""
+    row that an earlier entry names).  Rejected draft tokens stay reserved (``pages``)."""
     rows, lens = _pool_list(pool, rows, lens)
     device = _same_device(pool.arena, rows, lens)
     result = rows.new_empty(rows.shape)

@@ -15,7 +15,14 @@ length in tokens of every request row, the block table the attention kernels rea
 
 ``kernels.resize_requests`` admits, grows and releases rows, ``kernels.fork_requests``
 forks them copy-on-write and ``kernels.compact_pages`` moves live pages to the lowest
-numbers.  They change the pool (and the cache) in stream order and share the arena's
+numbers.  A row's length counts what is reserved for it.  Where a verify step's drafts are
+rejected it stays ahead of the tokens that are kept: the host passes the kept lengths to the
+attention and asks the next step for the longer of its need and the present length (a
+shorter one is refused).  Such a row may be forked once no whole page of its length lies
+behind the kept tokens, ``kept >= length // block_tokens * block_tokens``, a step or two
+later; before that both rows would write one shared page.
+
+The operators change the pool (and the cache) in stream order and share the arena's
 workspace: calls on one pool must be ordered, on one stream or by events.
 """
 

@@ -116,3 +116,62 @@ def test_one_prompt_many_answers(cuda_lib, hq, h, prompt, query, block, sink, re
     close(shared.step([0, 1, 3], q, k, v, norm, groups=[1, 1, 1], prefix=[prompt] * 3),
           alone.step([0, 1, 3], q, k, v, norm))
     assert kernels.read_status(DEV) == 0
+
+
+@pytest.mark.parametrize("prompt", [700, 766, 1023])
+def test_forks_behind_rejected_drafts(cuda_lib, prompt):
+    """Verify steps whose drafts are partly rejected: lengths in the pool stay at what was
+    reserved, the kept ones are the host's; a fork waits until no whole page of the reserved
+    length lies behind the kept tokens."""
+    block, hq, h, query = 256, 8, 1, 4
+    layout = CacheLayout(block, kv_heads=h, config=make_config(4, 64, mtp=query - 1))
+    shared, alone = (Server(layout, 40, 4, prompt + 200) for _ in range(2))
+    angle = torch.arange(prompt + 200, dtype=torch.float64, device=DEV)[:, None] * torch.exp(
+        -math.log(1e6) * torch.arange(0, 64, 2, dtype=torch.float64, device=DEV) / 64)
+    shared.table = alone.table = torch.cat((angle.cos(), angle.sin()), 1).float()
+    gen = torch.Generator(device=DEV).manual_seed(prompt)
+    norm = [(1 + 0.1 * torch.randn(256, device=DEV, generator=gen)).bfloat16() for _ in range(2)]
+
+    def tokens(rows, count):
+        return [torch.randn(rows, count, heads, 256, device=DEV, generator=gen).bfloat16() for heads in (hq, h, h)]
+
+    def verify(s, rows, kept, qkv, prefix=None):
+        """One step at the kept lengths; the pool's own go no further than they must."""
+        have = s.pool.seq_lens[rows].tolist()
+        lens = [max(a, b + query) for a, b in zip(have, kept)]
+        assert kernels.resize_requests(s.pool, ints(rows), ints(lens)).tolist() == [1] * len(rows)
+        meta, _ = s.meta(rows, query)
+        meta.seq_lens = ints([k + query for k in kept])
+        pos = (meta.seq_lens.long()[:, None] - query + torch.arange(query, device=DEV))
+        meta.slot_mapping = (meta.block_tables.long().gather(1, pos // 128) * 128 + pos % 128).flatten()
+        q, k, v = (x.flatten(0, 1) for x in qkv)
+        q, k = kernels.qk_norm_rope(q, k, *norm, pos.flatten(), s.table)
+        qrot = kernels.rotate_store(k, v, s.rk, s.rv, s.history, meta.slot_mapping, meta.counts, layout, query=q)
+        out = torch.empty(q.shape[0], hq * 256, dtype=torch.bfloat16, device=DEV)
+        plan = None
+        if prefix is not None:
+            plan = kernels.prepare_shared_prefix(meta, ints([0] * len(rows)), ints([prefix] * len(rows)), layout, hq)
+        kernels.decode_attention(qrot, q, k, v, s.history, s.window, meta, layout, 1 / 16, 8, s.rv, out, shared=plan)
+        return out.view(len(rows), query, hq, 256)
+
+    q, k, v = tokens(1, prompt)
+    shared.step([0], q, k, v, norm)
+    for r in range(3):
+        alone.step([r], q, k, v, norm)
+    kept, waited = prompt, 0
+    while True:
+        qkv = tokens(1, query)
+        close(verify(shared, [0], [kept], qkv), verify(alone, [0, 1, 2], [kept] * 3, [x.repeat(3, 1, 1, 1) for x in qkv])[:1])
+        kept += 1  # three drafts rejected
+        reserved = int(shared.pool.seq_lens[0])
+        if kept >= reserved // block * block:
+            break
+        waited += 1
+    assert reserved == kept + 3 and waited == (0 if prompt == 700 else 1 if prompt == 766 else 0)
+    assert kernels.fork_requests(shared.pool, ints([0, 0]), ints([1, 2]), shared.history, shared.window).tolist() == [1, 1]
+    at = [kept] * 3
+    for accepted in ([1, 4, 2], [3, 1, 4], [4, 4, 1], [2, 3, 3]):
+        qkv = tokens(3, query)
+        close(verify(shared, [0, 1, 2], at, qkv, prefix=kept), verify(alone, [0, 1, 2], at, qkv))
+        at = [a + b for a, b in zip(at, accepted)]
+    assert kernels.read_status(DEV) == 0
