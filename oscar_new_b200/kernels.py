@@ -618,10 +618,11 @@ def prepare_shared_prefix(meta, groups, prefix_lens, layout, hq, shared=None):
         raise ValueError("the plan was made for other heads, another layout or fewer requests")
     elif reqs < shared.max_reqs:
         raise ValueError(f"groups and prefix_lens must have the plan's {shared.max_reqs} entries")
-    for name in ("query_start_loc", "seq_lens", "counts"):
+    for name, size in (("query_start_loc", meta.num_reqs + 1), ("seq_lens", meta.num_reqs), ("counts", 2)):
         t = getattr(meta, name)
-        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 vector, got {tuple(t.shape)} {t.dtype}")
+        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or t.shape[0] < size:
+            raise ValueError(f"{name} must be a contiguous int32 vector of {size} entries or more, "
+                             f"got {tuple(t.shape)} {t.dtype}")
     table = meta.block_tables
     device = _same_device(groups, prefix_lens, shared.plan, meta.query_start_loc, meta.seq_lens, meta.counts, table)
     if reqs == 0:  # a new plan of an empty step: it shares nothing as it is
@@ -654,8 +655,8 @@ def _decode_shared(qrot, query, key, value, history, window, meta, layout, scale
     if key.shape != (n, layout.kv_heads, 256) or value.shape != key.shape:
         raise ValueError("key and value must be [n, KV heads, 256]")
     table = meta.block_tables
-    if table.stride(1) != 1:
-        raise ValueError("block table rows must be contiguous")
+    if table.stride(1) != 1 or table.shape[0] < meta.num_reqs:
+        raise ValueError("the block table must have a contiguous row per request")
     device = _same_device(qrot, query, key, value, history, window, rv, output, shared.plan, table,
                           meta.query_start_loc, meta.seq_lens, meta.counts, meta.tasks, meta.task_count,
                           None if scratch is None else scratch.partials)

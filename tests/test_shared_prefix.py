@@ -143,3 +143,18 @@ def test_windows_other_than_the_caches_are_refused(window):
 def test_a_history_of_another_type_is_refused():
     with pytest.raises(ValueError, match="whole contiguous pages"):
         kernels.decode_attention(**{**decode_args(), "history": torch.zeros(LAYOUT.stripe_page_bytes, dtype=torch.bfloat16)})
+
+
+@pytest.mark.parametrize("name,rows", [("query_start_loc", 3), ("seq_lens", 2), ("counts", 1)])
+def test_metadata_of_fewer_requests_is_refused_by_the_plan(name, rows):
+    ok, m = torch.zeros(3, dtype=torch.int32), meta()
+    setattr(m, name, getattr(m, name)[:rows])
+    with pytest.raises(ValueError, match=name):
+        kernels.prepare_shared_prefix(m, ok, ok, LAYOUT, 24)
+
+
+def test_block_tables_of_fewer_requests_are_refused():
+    a = decode_args()
+    a["meta"].block_tables = a["meta"].block_tables[:2]
+    with pytest.raises(ValueError, match="block table"):
+        kernels.decode_attention(**a)
