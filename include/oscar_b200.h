@@ -343,7 +343,7 @@ int oscar_page_pool_layout(int32_t num_pages, int32_t max_reqs, int32_t columns,
  * parent's tokens, sharing its full pages but the first (their counts grow by one); the
  * first page (its used slots and the request's BF16 window) and a partial last page (its
  * used slots) are copied to fresh pages.  history / window: the cache stripes of num_pages
- * pages.  A pair is valid when the parent had tokens and the child none before the call
+ * pages.  The lists lie outside the arena.  A pair is valid when the parent had tokens and the child none before the call
  * and no earlier pair names the child.  result[i] = 1 forked, 0 not forked because the
  * free pages ran out at this pair or before, -1 not a valid pair. */
 int oscar_fork_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, const int32_t *parents,
@@ -351,7 +351,8 @@ int oscar_fork_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int
                         int32_t *result, void *stream);
 
 /* Row rows[i] gets lens[i] tokens, i < count <= max_reqs: 0 releases the row (the counts of
- * its pages drop by one), a length not below the present one adds the missing pages.  All
+ * its pages drop by one), a length not below the present one adds the missing pages.  The
+ * lists lie outside the arena.  All
  * releases of the call come before any growth.  result[i] = 1 done, 0 unchanged because the
  * free pages ran out at this entry or before, -1 refused: row or length out of range, a
  * shorter length other than 0, or a row that an earlier entry names. */

@@ -395,7 +395,10 @@ def _pool_list(pool, *lists):
             raise ValueError("row lists are int32 [count], all of one length")
     if lists[0].shape[0] > pool.max_reqs:
         raise ValueError(f"{lists[0].shape[0]} entries for a pool of {pool.max_reqs} rows")
-    return [_dense(t) for t in lists]
+    # a view of the pool's own state counts as it is before the call
+    first = pool.arena.data_ptr()
+    last = first + 4 * pool.arena.numel()
+    return [t.clone() if first <= t.data_ptr() < last else _dense(t) for t in lists]
 
 
 def fork_requests(pool, parents, children, history, window):

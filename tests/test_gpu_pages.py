@@ -222,3 +222,17 @@ def test_long_rows(cuda_lib, block, columns, pages):
         p.fork([rng.randint(0, 6) for _ in range(3)], [rng.randint(0, 6) for _ in range(3)])
         if rng.random() < 0.5:
             p.compact()
+
+
+def test_lists_that_are_views_of_the_pool(cuda_lib):
+    """Every row takes its neighbour's length: the list is the pool's own length vector, and
+    counts as it was before the call."""
+    layout = CacheLayout(256, kv_heads=1, config=make_config(4, 64))
+    p = Pair(4000, 1400, 512, layout)
+    for spread in (0, 300):
+        p.resize(list(range(1400)), [0] * 1400)
+        p.resize(list(range(1400)), [100 + spread * (i < 700) - i // 14 for i in range(1400)])
+        rows, lens = list(range(1, 1400)), p.pool.seq_lens.tolist()[:1399]
+        got = kernels.resize_requests(p.pool, p.ints(rows), p.pool.seq_lens[:1399])
+        assert got.tolist() == p.model.resize(rows, lens)
+        p.state()
