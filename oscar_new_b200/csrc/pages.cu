@@ -13,7 +13,7 @@
 // Bytes: a page's used slots (tokens * H * 160, contiguous in the K stripe) and, for a
 // first page, the window (contiguous in the V stripe) are moved as 16 KiB slices: 131 MB (most of
 // it written) of 60 forks in 28 us, 4.6 TB/s, behind 8 us of decisions; 145 MB of a compaction
-// in 24 us.  The next slice's job fetched ahead of this one's stores: 28 us too, not kept.
+// in 26 us.  The next slice's job fetched ahead of this one's stores: 28 us too, not kept.
 #include <algorithm>
 
 #include "common.cuh"
