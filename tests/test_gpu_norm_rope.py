@@ -208,3 +208,18 @@ def test_infinities_reach_what_the_formula_says(cuda_lib, interleaved, value):
     check(ko, formula(q[:, 1:2], w, 0.0, 1e-6, tab[pos], rotary, interleaved))
     for t, d in enumerate(at):
         assert int(torch.isnan(qo[t, 1]).sum()) == (2 if d < rotary else 1)
+
+
+def test_rows_beyond_32_bits(cuda_lib):
+    n, hq = 360000, 24
+    assert n * hq * 256 > 2**31
+    q = torch.empty(n, hq, 256, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(n, 1, 256, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    some = torch.tensor([0, 1, 174762, 174763, 349525, 349526, n - 2, n - 1], device=DEV)
+    q[some] = torch.randn(len(some), hq, 256, device=DEV, generator=g).bfloat16()
+    k[some] = torch.randn(len(some), 1, 256, device=DEV, generator=g).bfloat16()
+    w, tab, pos = torch.ones(256, device=DEV), table(1000, 64), torch.arange(n, device=DEV) % 1000
+    qo, ko = kernels.qk_norm_rope(q, k, w, w, pos, tab)
+    check(qo[some], formula(q[some], w, 0.0, 1e-6, tab[pos[some]], 64, False))
+    check(ko[some], formula(k[some], w, 0.0, 1e-6, tab[pos[some]], 64, False))

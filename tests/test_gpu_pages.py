@@ -236,3 +236,32 @@ def test_lists_that_are_views_of_the_pool(cuda_lib):
         got = kernels.resize_requests(p.pool, p.ints(rows), p.pool.seq_lens[:1399])
         assert got.tolist() == p.model.resize(rows, lens)
         p.state()
+
+
+def test_pages_beyond_32_bits(cuda_lib):
+    """Fork and compaction of pages more than 2^31 bytes into the stripes."""
+    layout = CacheLayout(768, kv_heads=4, config=make_config(64, 256, 3))
+    pages, size = 1500, layout.stripe_page_bytes
+    assert 1400 * size > 2**31
+    pool = PagePool(pages, 4, 24, layout, DEV)
+    history = torch.zeros(pages * size, dtype=torch.uint8, device=DEV)
+    window = torch.zeros(pages * size // 2, dtype=torch.bfloat16, device=DEV)
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool.refcounts[1:1400] = 1  # all low pages are held by someone
+    assert kernels.resize_requests(pool, i(2), i(1000)).tolist() == [1]
+    assert pool.block_tables[2, :12:6].tolist() == [1400 * 6, 1401 * 6]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    h, w = history.view(pages, -1), window.view(torch.int16).view(pages, -1)
+    h[1400:1402] = torch.randint(0, 256, (2, size), dtype=torch.uint8, device=DEV, generator=g)
+    w[1400] = torch.randint(-2**15, 2**15, (size // 2,), dtype=torch.int16, device=DEV, generator=g)
+    used = [768 * 4 * 160, 232 * 4 * 160]
+    first, last, win = h[1400, :used[0]].clone(), h[1401, :used[1]].clone(), w[1400, :layout.window_page_bytes // 2].clone()
+    assert kernels.fork_requests(pool, i(2), i(0), history, window).tolist() == [1]
+    assert torch.equal(h[1402, :used[0]], first) and torch.equal(h[1403, :used[1]], last)
+    assert torch.equal(w[1402, :win.numel()], win) and not h[1403, used[1]:].any() and not w[1403].any()
+    pool.refcounts[1:1400] = 0
+    kernels.resize_requests(pool, i(2), i(0))
+    summary, to = kernels.compact_pages(pool, history, window)
+    assert summary.tolist() == [2, 2] and to[1402:1404].tolist() == [1, 2]
+    assert torch.equal(h[1, :used[0]], first) and torch.equal(h[2, :used[1]], last) and torch.equal(w[1, :win.numel()], win)
+    assert pool.block_tables[0, :12:6].tolist() == [6, 12]

@@ -557,3 +557,34 @@ def test_plan_of_the_most_requests(cuda_lib):
     assert torch.equal(torch.bincount(items[:, 0].long() // 2, minlength=n // 2), used[::2].long())
     assert torch.equal(used[::2], used[1::2]) and bool((items[:, 2] == 12).all()) and bool((items[:, 6] == 130).all())
     assert torch.equal(items[:, 3], items[:, 0])
+
+
+@pytest.mark.parametrize("members,prefix,query,hq,h", [(3, 700, 1, 64, 1), (4, 600, 1, 16, 16), (5, 800, 4, 16, 1)])
+def test_head_layouts_at_the_ends(cuda_lib, members, prefix, query, hq, h):
+    b = simple(members, prefix, lambda i: 40 * i, query, hq, h, seed=30 + hq + h)
+    b.check(b.run())
+    assert min(b.plan_words()[1][:members]) > 4
+
+
+@pytest.mark.parametrize("parts,own", [(63, 1), (1, 63), (32, 64)])
+def test_most_and_fewest_splits(cuda_lib, parts, own):
+    b = simple(3, 6000, lambda i: 2500 * i, 1, 8, 1, seed=31)
+    plan = kernels.SharedPrefix(3, 3, 8, b.layout, DEV, splits=parts)
+    kernels.prepare_shared_prefix(b.meta, b.groups, b.lens, b.layout, 8, shared=plan)
+    b.check(b.run(shared=plan, splits=own))
+    assert b.plan_words()[2][:3] == [max(it[7] for it in b.plan_words()[0]) + 1] * 3 and max(b.plan_words()[2]) <= parts
+
+
+def test_two_steps_at_once_on_two_streams(cuda_lib):
+    """Own plans, scratch and outputs; the library's side stream is common to both."""
+    steps = [simple(12, 2000 + 300 * i, lambda j: 7 * j, 1, 24, 4, seed=32 + i) for i in range(2)]
+    want = [b.run().clone() for b in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, (b, stream) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(b.run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i]) and kernels.read_status(DEV) == 0
