@@ -335,27 +335,28 @@ int oscar_decode_attention_shared(const void *qrot, const void *query, int64_t q
  * 128-token kernel blocks (unused entries 0), then workspace that the calls below share,
  * so calls on one arena must be ordered.  A row of L tokens holds ceil(L / block_tokens)
  * pages; fresh pages are the free pages of the lowest numbers, handed out in list order:
- * results depend on the state and the list alone.  max_reqs * columns < 2^31.  Writes the word offsets {counts,
- * lengths, table, end of the state, total words} to offsets[0..4]. */
+ * results depend on the state and the list alone.  max_reqs * columns < 2^31.  Writes the
+ * word offsets {counts, lengths, table, end of the state, total words} to offsets[0..4]. */
 int oscar_page_pool_layout(int32_t num_pages, int32_t max_reqs, int32_t columns, int64_t *offsets);
 
 /* Fork row children[i] from row parents[i], i < count <= max_reqs: the child holds the
  * parent's tokens, sharing its full pages but the first (their counts grow by one); the
  * first page (its used slots and the request's BF16 window) and a partial last page (its
  * used slots) are copied to fresh pages.  history / window: the cache stripes of num_pages
- * pages.  The lists lie outside the arena.  A pair is valid when the parent had tokens and the child none before the call
- * and no earlier pair names the child.  result[i] = 1 forked, 0 not forked because the
- * free pages ran out at this pair or before, -1 not a valid pair. */
+ * pages.  The lists lie outside the arena.  A pair is valid when the parent had tokens and
+ * the child none before the call and no earlier pair names the child.  result[i] = 1 forked,
+ * 0 not forked because the free pages ran out at this pair or before, -1 not a valid pair.
+ * Tokens count as the row's length says: see pages.py for parents with rejected drafts. */
 int oscar_fork_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, const int32_t *parents,
                         const int32_t *children, int32_t count, void *history, void *window, oscar_geometry geo,
                         int32_t *result, void *stream);
 
 /* Row rows[i] gets lens[i] tokens, i < count <= max_reqs: 0 releases the row (the counts of
  * its pages drop by one), a length not below the present one adds the missing pages.  The
- * lists lie outside the arena.  All
- * releases of the call come before any growth.  result[i] = 1 done, 0 unchanged because the
- * free pages ran out at this entry or before, -1 refused: row or length out of range, a
- * shorter length other than 0, or a row that an earlier entry names. */
+ * lists lie outside the arena.  All releases of the call come before any growth.
+ * result[i] = 1 done, 0 unchanged because the free pages ran out at this entry or before,
+ * -1 refused: row or length out of range, a shorter length other than 0, or a row that an
+ * earlier entry names. */
 int oscar_resize_requests(int32_t *arena, int32_t num_pages, int32_t max_reqs, int32_t columns, int32_t block_tokens,
                           const int32_t *rows, const int32_t *lens, int32_t count, int32_t *result, void *stream);
 

@@ -439,8 +439,9 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Pool p
   }
 }
 
-// used[page] = most tokens a request keeps in a page (0: no request does), list[page] = 1 when a request starts
-// in it (its window), both by the old page numbers; the table's blocks follow their pages
+// used[page] = most tokens a request keeps in a page (0: no request does), list[page] = 1
+// when a request starts in it (its window), both by the old page numbers; the table's blocks
+// follow their pages
 __global__ void __launch_bounds__(kCopyThreads) compact_rows_kernel(const Pool p) {
   const int r = blockIdx.x;
   const int n = (int)min((int64_t)max(p.lens[r], 0), row_tokens(p));
